@@ -116,7 +116,10 @@ def build_kernels(verbose: bool = False, force: bool = False, jobs: int = 8, def
     hipcc = _hipcc()
     # -amdgpu-mfma-vgpr-form: MFMA accumulators in arch VGPRs (gfx950 has one unified 512-entry
     # file per SIMD); with AGPR accumulators hipcc shuttled them AGPR<->VGPR inside the K1 loop.
+    # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, some forms of which have given wrong values now and then
+    # (the host pass warns that it does not know the feature).
     flags = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-munsafe-fp-atomics",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-mllvm", "-amdgpu-mfma-vgpr-form=1", "-Wno-unused-result", f"-I{CSRC / 'kernels'}",
              *[f"-D{d}" for d in defines]]
 
