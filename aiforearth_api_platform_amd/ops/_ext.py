@@ -74,6 +74,12 @@ _SIGS = {
     "ai4e_gn_relu_head8": [_vp, _c_int, _c_int, _vp, _vp, _c_int, _vp, _vp, _c_int, _c_int, _vp],
     "ai4e_conv3x3_tile_fwd": [_vp, _vp, _vp, _vp, _c_int, _vp] + [_c_int] * 10 + [_vp, _c_int, _vp],
     "ai4e_jpeg_decode": [_vp, _c_int, _c_int, _c_int, _c_long, _c_long, _c_int, _vp],
+    "ai4e_mx_quantize": [_vp, _c_long, _c_long, _c_int, _c_int, _c_int, _vp, _vp, _vp],
+    "ai4e_mx_dequantize": [_vp, _vp, _c_long, _c_int, _c_int, _c_int, _vp, _vp],
+    "ai4e_mx_linear": [_vp, _vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp],
+    "ai4e_rms_norm_mx8": [_vp, _c_long, _vp, _c_long, _vp, _c_float, _c_long, _c_int, _c_int, _vp, _vp, _vp, _vp],
+    "ai4e_label_logprobs_ws": [_c_long, _c_int, _c_int],
+    "ai4e_label_logprobs": [_vp, _c_long, _c_long, _c_int, _c_int, _vp, _c_int, _c_int, _c_int] + [_vp] * 6,
     "ai4e_crumbs_alloc": [_c_int, _vp, _vp],
     "ai4e_crumb": [_vp, _c_int, _vp],
 }
@@ -127,6 +133,22 @@ def has(name: str) -> bool:
 
 def stream_ptr(device: Optional[torch.device] = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with the stream that is current on ``device``, also while another device is current (a launch goes to
+    the current device, whatever its stream)."""
+    if torch.cuda.current_device() == device.index:
+        call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def refuse_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """For operators with no backward pass: a call that autograd would have to record is an error."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -3,14 +3,17 @@
 ``softmax_topk(logits, k)`` -> ``(idx int32 [N,k], prob fp32 [N,k])``, sorted by descending probability,
 ties to the lower class index. Replaces cast + ``torch.softmax`` + ``torch.topk`` (+ sort + index cast):
 five launches in the serving engine's graph tail. The PyTorch path is the reference.
+
+``label_logprobs(logits, labels, k)`` (``csrc/kernels/logprobs.hip``): the log-probability of given labels, the entropy
+and the k most likely classes, over any number of classes.
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
-from . import _ext
+from . import _ext, mx
 
 
 def softmax_topk(logits: torch.Tensor, k: int = 5) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -23,3 +26,75 @@ def softmax_topk(logits: torch.Tensor, k: int = 5) -> Tuple[torch.Tensor, torch.
     _ext.call("ai4e_softmax_topk", logits.data_ptr(), logits.stride(0), n, c, k, idx.data_ptr(), prob.data_ptr(),
               _ext.stream_ptr(logits.device))
     return idx, prob
+
+
+class LabelLogprobs(NamedTuple):
+    logp: Optional[torch.Tensor]  # fp32, labels' shape; None without labels
+    entropy: torch.Tensor         # fp32 [...], in nats
+    top_idx: torch.Tensor         # int32 [..., k]
+    top_logp: torch.Tensor        # fp32 [..., k], descending
+
+
+MAX_ALTERNATIVES = 64
+
+
+def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, k: int = 5) -> LabelLogprobs:
+    """``logits`` [..., C] (bf16, fp16 or fp32; rows may be strided), ``labels`` [...] or [..., L] (int64 or int32) and
+    ``0 <= k <= 64`` alternatives, ties to the lower class.
+
+    A masked class has the logit -inf: its log-probability is -inf, it adds nothing to the entropy and is no alternative
+    (where fewer than k classes are left, the rest are class -1 at -inf). A row with nothing left has log-probabilities
+    -inf and entropy 0. A row with a NaN or +inf has no distribution: NaN, classes -1. A negative label means that the
+    row has none: 0, so that sums pass over it; one of C or more gives NaN. No backward pass."""
+    c = logits.shape[-1] if logits.dim() else 0
+    if logits.dtype not in mx.DTYPE_CODE or c == 0:
+        raise ValueError("label_logprobs expects bfloat16, float16 or float32 logits of at least one class")
+    if not 0 <= k <= min(c, MAX_ALTERNATIVES):
+        raise ValueError(f"label_logprobs: k is 0 to {min(c, MAX_ALTERNATIVES)}, not {k}")
+    lead = logits.shape[:-1]
+    if labels is not None:
+        if labels.dtype not in (torch.int64, torch.int32) or labels.device != logits.device:
+            raise ValueError("label_logprobs: labels are int64 or int32, on the logits' device")
+        if labels.shape != lead and labels.shape[:-1] != lead:
+            raise ValueError(f"label_logprobs: labels {tuple(labels.shape)} fit no logits {tuple(logits.shape)}")
+    _ext.refuse_grad("label_logprobs", logits)
+    n_labels = 0 if labels is None else 1 if labels.shape == lead else labels.shape[-1]
+    if _ext.backend_for(logits) != "hip":
+        return _label_logprobs_reference(logits, labels, n_labels, k)
+    dev = logits.device
+    logp = None if labels is None else torch.empty(labels.shape, device=dev, dtype=torch.float32)
+    entropy = torch.empty(lead, device=dev, dtype=torch.float32)
+    top_idx = torch.empty(*lead, k, device=dev, dtype=torch.int32)
+    top_logp = torch.empty(*lead, k, device=dev, dtype=torch.float32)
+    x = mx.rows_2d(logits)
+    rows = x.shape[0]
+    if rows:
+        labels = None if labels is None else labels.contiguous()
+        words = _ext.call_int("ai4e_label_logprobs_ws", rows, c, k)
+        ws = torch.empty(words, device=dev, dtype=torch.float32) if words else None
+        _ext.call_on(dev, "ai4e_label_logprobs", x.data_ptr(), max(x.stride(0), c), rows, c, mx.DTYPE_CODE[x.dtype],
+                     _ext.ptr(labels) if n_labels else None, int(n_labels > 0 and labels.dtype == torch.int64), n_labels, k,
+                     _ext.ptr(logp), entropy.data_ptr(), top_idx.data_ptr(), top_logp.data_ptr(), _ext.ptr(ws))
+    return LabelLogprobs(logp, entropy, top_idx, top_logp)
+
+
+def _label_logprobs_reference(logits, labels, n_labels, k) -> LabelLogprobs:
+    c = logits.shape[-1]
+    x = logits.float().reshape(-1, c)
+    nan = torch.full((), float("nan"), device=x.device)
+    bad = ~(x < float("inf")).all(1)
+    none = torch.isneginf(x).all(1) & ~bad
+    lp = torch.log_softmax(x.double(), 1)
+    lp = torch.where(none[:, None], torch.full_like(lp, -float("inf")), torch.where(bad[:, None], nan.double(), lp))
+    term = torch.where(torch.isneginf(lp), torch.zeros_like(lp), lp.exp() * lp)
+    entropy = (0.0 - term.sum(1)).float()
+    order = torch.sort(torch.where(bad[:, None], torch.zeros_like(x), x), dim=1, descending=True, stable=True).indices[:, :k]
+    top = lp.gather(1, order)
+    idx = torch.where(torch.isneginf(top) | bad[:, None], torch.full_like(order, -1), order).to(torch.int32)
+    logp = None if labels is None else torch.empty(labels.shape, device=x.device)
+    if n_labels:
+        lab = labels.reshape(-1, n_labels).long()
+        logp = lp.gather(1, lab.clamp(0, c - 1))
+        logp = torch.where(lab < 0, torch.zeros_like(logp), torch.where(lab >= c, nan.double(), logp)).float().view(labels.shape)
+    lead = logits.shape[:-1]
+    return LabelLogprobs(logp, entropy.view(lead), idx.view(*lead, k), top.float().view(*lead, k))

@@ -1,12 +1,13 @@
-"""GroupNorm (+ReLU) [K2] and bilinear 2x upsample [K3] on NHWC tensors, with concat-slice outputs."""
+"""GroupNorm (+ReLU) [K2] and bilinear 2x upsample [K3] on NHWC tensors, with concat-slice outputs; RMS norm with the
+residual's addition, written as MX e4m3."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 import torch.nn.functional as F
 
-from . import _ext
+from . import _ext, mx
 
 _GN_CHUNK = []
 
@@ -143,3 +144,36 @@ def upsample2x_nhwc(x: torch.Tensor, out: Optional[torch.Tensor] = None, out_cof
     y = F.interpolate(x.permute(0, 3, 1, 2).float(), scale_factor=2, mode="bilinear", align_corners=False)
     out[..., out_coff:out_coff + c] = y.permute(0, 2, 3, 1).to(out.dtype)
     return out
+
+
+def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6) -> Tuple[mx.MxTensor, Optional[torch.Tensor]]:
+    """``h = x + residual``; ``h / sqrt(mean(h^2) + eps) * gamma`` over the last axis, as MX e4m3 activations for
+    ``mx.mx_linear`` (csrc/kernels/rms_norm.hip). ``x`` and ``residual`` [..., C] in bf16, fp16 or fp32 (rows may be
+    strided), ``gamma`` [C] (kept in float32 by a caller that wants no cast per call). Returns the MxTensor and ``h`` in
+    x's type, for the next residual (None without ``residual``); the norm is taken of the sum before that rounding."""
+    c = x.shape[-1] if x.dim() else 0
+    if x.dtype not in mx.DTYPE_CODE or c == 0:
+        raise ValueError("rms_norm_mx8 expects bfloat16, float16 or float32 with a last axis of at least one value")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("rms_norm_mx8: residual has to have x's shape and type")
+    if tuple(gamma.shape) != (c,) or not gamma.is_floating_point():
+        raise ValueError(f"rms_norm_mx8: gamma is a floating tensor of {c} values")
+    if gamma.device != x.device or (residual is not None and residual.device != x.device):
+        raise ValueError("rms_norm_mx8: x, gamma and residual have to be on one device")
+    if not eps > 0:
+        raise ValueError("rms_norm_mx8: eps has to be positive")
+    _ext.refuse_grad("rms_norm_mx8", x, gamma, residual)
+    if _ext.backend_for(x) != "hip":
+        h = x.float() if residual is None else x.float() + residual.float()
+        y = h.double() / torch.sqrt(h.double().square().mean(-1, keepdim=True) + eps) * gamma.double()
+        return mx.quantize_reference(y.float(), "e4m3"), None if residual is None else h.to(x.dtype)
+    q = mx.empty(x.shape[:-1], c, "e4m3", x.device)
+    h = None if residual is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    g32 = gamma.to(torch.float32).contiguous()
+    x2 = mx.rows_2d(x)
+    r2 = None if residual is None else mx.rows_2d(residual)
+    _ext.call_on(x.device, "ai4e_rms_norm_mx8", x2.data_ptr(), max(x2.stride(0), c), _ext.ptr(r2),
+                 0 if r2 is None else max(r2.stride(0), c), g32.data_ptr(), eps, x2.shape[0], c, mx.DTYPE_CODE[x.dtype],
+                 _ext.ptr(h), q.data.data_ptr(), q.scale.data_ptr())
+    return q, h

@@ -1,0 +1,151 @@
+// RMS norm with the residual's addition, written as MX e4m3 (formats: mx.h).
+//
+//   h = x + residual            y = h / sqrt(mean(h^2) + eps) * gamma            (e4m3, scales) = mx(y), h kept
+//
+// One workgroup per row. The row stays in registers between the sum of squares and the products, so memory is what
+// bounds it: per value 2 + 2 B in, 2 B (h) and 1.03 B (codes, scales) out for 16-bit rows.
+// A value next to the border of two 8-bit neighbours falls to either side by the last bit of y, so y is computed to
+// one rounding: the row's factor as a double, split into a float and its remainder, and h * factor with its error.
+#include "mx.h"
+
+namespace {
+
+// sum over the workgroup's WAVES waves of a per-lane float (each lane's own sum has at most a row's share of squares),
+// added in double
+template <int WAVES>
+__device__ __forceinline__ double row_sum(float v, double* lds) {
+  double s = v;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if constexpr (WAVES > 1) {
+    __syncthreads();  // the last row's sums have been read
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s += lds[w];
+  }
+  return s;
+}
+
+template <int DT>
+__device__ __forceinline__ void load_h(const typename mx_elem<DT>::type* x, const typename mx_elem<DT>::type* r, int n,
+                                       float (&h)[8]) {
+  if (n >= 8) {
+    mx_floats<DT>(mx_load8<DT>(x), h);
+    if (r) {
+      float g[8];
+      mx_floats<DT>(mx_load8<DT>(r), g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] += g[i];
+    }
+  } else {
+    mx_load8_tail<DT>(x, n, 0.f, h);
+    if (r) {
+      float g[8];
+      mx_load8_tail<DT>(r, n, 0.f, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] += g[i];
+    }
+  }
+}
+
+// CH > 0: the row's chunks of 8 per lane, kept in registers; CH == 0: any width, read a second time
+template <int DT, int WAVES, int CH>
+__global__ __launch_bounds__(WAVES * 64) void rms_norm_mx8_kernel(
+    const typename mx_elem<DT>::type* __restrict__ x, long ldx, const typename mx_elem<DT>::type* __restrict__ res,
+    long ldr, const float* __restrict__ gamma, float eps, long rows, int c, int cp,
+    typename mx_elem<DT>::type* __restrict__ hout, uint8_t* __restrict__ data, uint8_t* __restrict__ scale) {
+  constexpr int T = WAVES * 64;
+  constexpr int KEEP = CH > 0 ? CH : 1;
+  __shared__ double lds[WAVES];
+  const int tid = threadIdx.x;
+  const int nch = CH > 0 ? CH : (cp / 8 + T - 1) / T;
+  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const auto* xr = x + row * ldx;
+    const auto* rr = res ? res + row * ldr : nullptr;
+    float h[KEEP][8];
+    float sq = 0.f;
+#pragma unroll
+    for (int j = 0; j < nch; ++j) {
+      const int col = (j * T + tid) * 8;
+      float(&v)[8] = h[CH > 0 ? j : 0];
+      load_h<DT>(xr + col, rr ? rr + col : nullptr, c - col, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
+      if (hout && col < c) mx_store8<DT>(hout + row * c + col, v, c - col);
+    }
+    double ms = row_sum<WAVES>(sq, lds);
+    double factor;
+    if (ms < 3e38) {
+      factor = 1.0 / sqrt(ms / c + static_cast<double>(eps));
+    } else {  // the squares left 32 bits (or are not finite): once more, scaled by 2^-80
+      sq = 0.f;
+#pragma unroll
+      for (int j = 0; j < nch; ++j) {
+        const int col = (j * T + tid) * 8;
+        float(&v)[8] = h[CH > 0 ? j : 0];
+        if (CH == 0) load_h<DT>(xr + col, rr ? rr + col : nullptr, c - col, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float u = v[i] * 0x1p-80f;
+          sq = fmaf(u, u, sq);
+        }
+      }
+      ms = row_sum<WAVES>(sq, lds);
+      factor = 1.0 / (sqrt(ms / c + static_cast<double>(eps) * 0x1p-160) * 0x1p80);
+    }
+    const float fh = static_cast<float>(factor), fl = static_cast<float>(factor - static_cast<double>(fh));
+#pragma unroll
+    for (int j = 0; j < nch; ++j) {
+      const int col = (j * T + tid) * 8;
+      if (col >= cp) break;  // cp is a multiple of 128: a block's four lanes leave together
+      float(&v)[8] = h[CH > 0 ? j : 0];
+      if (CH == 0) load_h<DT>(xr + col, rr ? rr + col : nullptr, c - col, v);
+      float g[8], y[8];
+      if (col + 8 <= c)
+        mx_floats<MX_F32>(mx_load8<MX_F32>(gamma + col), g);
+      else
+        mx_load8_tail<MX_F32>(gamma + col, c - col, 0.f, g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float a = v[i] * fh, e = fmaf(v[i], fl, fmaf(v[i], fh, -a));
+        y[i] = col + i < c ? fmaf(a, g[i], e * g[i]) : 0.f;  // also where the factor is not finite
+      }
+      const int code = mx_scale_code<MX_E4M3>(mx_quad_max(mx_abs_bits8(y)));
+      const long at = row * cp + col;
+      *reinterpret_cast<uint2*>(data + at) = mx_pack_e4m3(y, code);
+      if ((tid & 3) == 0) scale[at >> 5] = static_cast<uint8_t>(code);
+    }
+  }
+}
+
+}  // namespace
+
+// x [rows, ldx] and residual [rows, ldr] (or null) of type dt (0 bf16, 1 fp16, 2 fp32), c valid columns; gamma [c] fp32;
+// hout [rows, c] of type dt (or null); data [rows, cp], scale [rows, cp / 32], cp = c up to a multiple of 128.
+AI4E_API int ai4e_rms_norm_mx8(const void* x, long ldx, const void* residual, long ldr, const void* gamma, float eps,
+                               long rows, int c, int dt, void* hout, void* data, void* scale, hipStream_t s) {
+  if (!x || !gamma || !data || !scale || c <= 0 || c > (1 << 30) || rows < 0 || dt < 0 || dt > 2 || ldx < c ||
+      (residual && ldr < c) || !(eps > 0.f))
+    return AI4E_EINVAL;
+  if (rows == 0) return AI4E_OK;
+  const int cp = ai4e_cdiv(c, MX_ALIGN) * MX_ALIGN;
+  const dim3 grid(static_cast<unsigned>(rows < (1 << 20) ? rows : (1 << 20)));
+#define GO(DT, W, CH)                                                                                            \
+  hipLaunchKernelGGL((rms_norm_mx8_kernel<DT, W, CH>), grid, dim3(W * 64), 0, s,                                 \
+                     static_cast<const mx_elem<DT>::type*>(x), ldx, static_cast<const mx_elem<DT>::type*>(residual), \
+                     ldr, static_cast<const float*>(gamma), eps, rows, c, cp, static_cast<mx_elem<DT>::type*>(hout), \
+                     static_cast<uint8_t*>(data), static_cast<uint8_t*>(scale))
+#define PICK(DT)                  \
+  if (cp <= 512) GO(DT, 1, 1);    \
+  else if (cp <= 2048) GO(DT, 4, 1); \
+  else if (cp <= 8192) GO(DT, 8, 2); \
+  else GO(DT, 8, 0)
+  if (dt == MX_BF16) { PICK(MX_BF16); }
+  else if (dt == MX_F16) { PICK(MX_F16); }
+  else { PICK(MX_F32); }
+#undef PICK
+#undef GO
+  return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
+}
