@@ -1,59 +1,233 @@
 // y = x . w^T + bias over MX operands (formats: mx.h): x e4m3 or e2m1, w e2m1, both [rows, k].
+//
+// gfx950's block-scaled matrix instructions take both formats and their scales as they lie in memory. The rows of w are
+// the first operand and the rows of x the second, so a lane ends with four consecutive outputs of one row of x.
+//
+// v_mfma_scale_f32_32x32x64: D[32 x 32] += A[32 x 64] . B[32 x 64]^T, a scale for each row and block of 32 (measured):
+//   lane l holds row l & 31; its 32 elements are k = 32 (l >> 5) .. + 31 of e2m1, and 16 (l >> 5) .. + 15 and
+//   32 + 16 (l >> 5) .. + 15 of e4m3; its scale is that of block l >> 5 in both
+//   of D it holds column l & 31 (a row of x), rows 8 (i >> 2) + 4 (l >> 5) + (i & 3), i = 0..15 (rows of w)
+// Operands of registers alone run at 4.4 PFLOP/s with e4m3 on one side and 8.0 with e2m1 on both, whose 32 x 32 x 64
+// form is twice as fast as the 16 x 16 x 128 one; hence the large tiles are made of it.
+#include "conv_common.h"
 #include "mx.h"
 
 namespace {
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
-// v_mfma_scale_f32_32x32x64: D[32 x 32] += A[32 x 64] . B[32 x 64]^T, a scale for each row and block of 32.
-// Lane l holds row l & 31. Its 32 elements are k = 32 (l >> 5) .. + 31 of e2m1, and k = 16 (l >> 5) .. + 15 and
-// 32 + 16 (l >> 5) .. + 15 of e4m3; its scale is that of block l >> 5 in both (measured).
-// Of D it holds column l & 31, rows 8 (i >> 2) + 4 (l >> 5) + (i & 3) for i = 0..15.
-template <int FMT>
-__device__ __forceinline__ i32x8_t load_frag(const uint8_t* row, int k0, int half) {
-  i32x8_t v = {};
-  if constexpr (FMT == MX_E4M3) {
-    const uint4 a = *reinterpret_cast<const uint4*>(row + k0 + 16 * half);
-    const uint4 b = *reinterpret_cast<const uint4*>(row + k0 + 32 + 16 * half);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4*>(row + (k0 >> 1) + 16 * half);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  }
-  return v;
+// 16 B (4 B) per lane from base + off to LDS at (wave-uniform lds + 16 (4) * lane); completion is counted by vmcnt.
+// M0 is put back: the compiler reserves it.
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
+  uint32_t keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(off), "s"(base), "s"(lds)
+      : "memory");
+}
+__device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t lds) {
+  uint32_t keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, %2\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(off), "s"(base), "s"(lds)
+      : "memory");
 }
 
-// one 32 x 32 tile of y per wave: rows of w are the matrix instruction's first operand, so a lane ends with four
-// consecutive outputs of one row of x
-template <int FX, int DT>
-__global__ __launch_bounds__(256) void mx_linear_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs,
-                                                        const uint8_t* __restrict__ w, const uint8_t* __restrict__ ws,
-                                                        const float* __restrict__ bias, int m, int n, int kp,
-                                                        typename mx_elem<DT>::type* __restrict__ y) {
+// Rows of a tile in LDS, 128 elements each: 128 B (e4m3) or 64 B (e2m1). A DMA writes 1024 consecutive bytes, 8 or 16
+// rows; the 16-B chunks of a row are permuted by the row so that the fragment reads of neighbouring rows fall into
+// different banks, which is done by permuting the source addresses.
+template <int FMT>
+struct TileRow {
+  static constexpr int BYTES = FMT == MX_E4M3 ? 128 : 64, CHUNKS = BYTES / 16, PER_DMA = 1024 / BYTES;
+  static __device__ __forceinline__ int swizzle(int row) { return FMT == MX_E4M3 ? row & 7 : ai4e_conv::swz(row); }
+};
+
+// The tile kernel: BX x BW outputs per workgroup, WX x WW waves of TX x TW fragments of 32 x 32. Steps of 128 along k go
+// through a ring of STAGES stages in LDS, written by DMA STAGES - 1 steps ahead; a barrier per step. Fragments are read half a
+// step before the matrix instructions that take them.
+template <int FX, int DT, int WX, int WW, int TX, int TW, int STAGES>
+__global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
+    const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w,
+    const uint8_t* __restrict__ ws, const float* __restrict__ bias, int m, int n, int kp, int tiles_x, int tiles_w,
+    typename mx_elem<DT>::type* __restrict__ y) {
+  constexpr int NW = WX * WW, BX = WX * TX * 32, BW = WW * TW * 32;
+  typedef TileRow<FX> XR;
+  typedef TileRow<MX_E2M1> WR;
+  constexpr int X_BYTES = BX * XR::BYTES, W_BYTES = BW * WR::BYTES, S_BYTES = (BX + BW) * 4;
+  constexpr int STAGE = X_BYTES + W_BYTES + S_BYTES;
+  constexpr int X_DMA = X_BYTES / 1024 / NW, W_DMA = W_BYTES / 1024 / NW, S_DMA = (BX + BW) / 64;
+  constexpr int PER_STAGE = X_DMA + W_DMA + 1;
+  static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && S_DMA <= NW && BX % 64 == 0 && BW % 64 == 0, "");
+  static_assert(STAGE * STAGES <= 160 * 1024, "");
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int tiles_n = (n + 31) / 32;
-  const long tile = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  const int tm = static_cast<int>(tile / tiles_n), tn = static_cast<int>(tile % tiles_n);
-  if (tm * 32 >= m) return;
-  const int rx = min(tm * 32 + (lane & 31), m - 1), rw = min(tn * 32 + (lane & 31), n - 1);
-  const uint8_t* xr = x + static_cast<long>(rx) * (FX == MX_E4M3 ? kp : kp / 2);
-  const uint8_t* wr = w + static_cast<long>(rw) * (kp / 2);
-  const uint8_t* xsr = xs + static_cast<long>(rx) * (kp / 32);
-  const uint8_t* wsr = ws + static_cast<long>(rw) * (kp / 32);
-  f32x16_t acc = {};
-  for (int k0 = 0; k0 < kp; k0 += 64) {
-    const i32x8_t a = load_frag<MX_E2M1>(wr, k0, half), b = load_frag<FX>(xr, k0, half);
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 4, FX == MX_E4M3 ? 0 : 4, 0,
-                                                          wsr[(k0 >> 5) + half], 0, xsr[(k0 >> 5) + half]);
-  }
-  const int row = tm * 32 + (lane & 31);
-  if (row >= m) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // neighbouring workgroups of one XCD take tiles of a block of 4 rows of tiles, which shares x and w in its L2
+  const int t = xcd_remap(blockIdx.x, gridDim.x);
+  constexpr int GROUP = 4;
+  const int group = t / (GROUP * tiles_w), g0 = group * GROUP, gh = min(GROUP, tiles_x - g0);
+  const int in = t - group * GROUP * tiles_w;
+  const int x0 = (g0 + in % gh) * BX, w0 = (in / gh) * BW;
+
+  const int px = FX == MX_E4M3 ? kp : kp / 2, pw = kp / 2, ps = kp / 32;  // row pitches in bytes
+  uint32_t xoff[X_DMA], woff[W_DMA];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int col = tn * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
-    if (col < n) y[static_cast<long>(row) * n + col] = mx_elem<DT>::from(acc[i] + (bias ? bias[col] : 0.f));
+  for (int j = 0; j < X_DMA; ++j) {
+    const int row = (wave * X_DMA + j) * XR::PER_DMA + lane / XR::CHUNKS;
+    xoff[j] = static_cast<uint32_t>(min(row, m - 1 - x0)) * px + ((lane % XR::CHUNKS) ^ XR::swizzle(row)) * 16;
   }
+#pragma unroll
+  for (int j = 0; j < W_DMA; ++j) {
+    const int row = (wave * W_DMA + j) * WR::PER_DMA + lane / WR::CHUNKS;
+    woff[j] = static_cast<uint32_t>(min(row, n - 1 - w0)) * pw + ((lane % WR::CHUNKS) ^ WR::swizzle(row)) * 16;
+  }
+  const int sd = wave % S_DMA;  // a wave brings 64 rows' scales
+  const bool s_of_x = sd < BX / 64;
+  const int srow = s_of_x ? min(sd * 64 + lane, m - 1 - x0) : min((sd - BX / 64) * 64 + lane, n - 1 - w0);
+  const uint32_t soff = static_cast<uint32_t>(srow) * ps;
+  const uint8_t* xb = x + static_cast<long>(x0) * px;
+  const uint8_t* wb = w + static_cast<long>(w0) * pw;
+  const uint8_t* sb = s_of_x ? xs + static_cast<long>(x0) * ps : ws + static_cast<long>(w0) * ps;
+
+  const int nk = kp / MX_ALIGN;
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) uint8_t*)lds));
+  auto issue = [&](int kt, uint32_t slot) {  // past the end the last step is brought again, into a slot nobody reads
+    const int k = min(kt, nk - 1);
+    const uint32_t base = lds0 + slot * STAGE;
+#pragma unroll
+    for (int j = 0; j < X_DMA; ++j)
+      dma16(xb + static_cast<long>(k) * XR::BYTES, xoff[j], base + (wave * X_DMA + j) * 1024);
+#pragma unroll
+    for (int j = 0; j < W_DMA; ++j)
+      dma16(wb + static_cast<long>(k) * WR::BYTES, woff[j], base + X_BYTES + (wave * W_DMA + j) * 1024);
+    dma4(sb + static_cast<long>(k) * 4, soff, base + X_BYTES + W_BYTES + sd * 256);
+  };
+
+  const int wx = wave % WX, ww = wave / WX;
+  const int r = lane & 31;
+  const int xrow = wx * TX * 32 + r, wrow = ww * TW * 32 + r;
+  const int xa = xrow * XR::BYTES + (half ^ XR::swizzle(xrow)) * 16;
+  const int wa = X_BYTES + wrow * WR::BYTES + (half ^ WR::swizzle(wrow)) * 16;
+  const int xsa = X_BYTES + W_BYTES + xrow * 4, wsa = X_BYTES + W_BYTES + (BX + wrow) * 4;
+
+  i32x8_t fx[2][TX], fw[2][TW];
+  int sx[2][TX], sw[2][TW];
+  // fragments of half step u of a stage; the lane's scale bytes are 2 u + half of its row's four
+  auto read = [&](const uint8_t* st, int u, i32x8_t(&ax)[TX], i32x8_t(&aw)[TW]) {
+#pragma unroll
+    for (int i = 0; i < TX; ++i) {
+      if constexpr (FX == MX_E4M3) {
+        const i32x4_t a = *reinterpret_cast<const i32x4_t*>(st + (xa ^ (64 * u)) + i * 32 * XR::BYTES);
+        const i32x4_t b = *reinterpret_cast<const i32x4_t*>(st + (xa ^ (64 * u + 32)) + i * 32 * XR::BYTES);
+        ax[i] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+      } else {
+        const i32x4_t a = *reinterpret_cast<const i32x4_t*>(st + (xa ^ (32 * u)) + i * 32 * XR::BYTES);
+        ax[i] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < TW; ++j) {
+      const i32x4_t a = *reinterpret_cast<const i32x4_t*>(st + (wa ^ (32 * u)) + j * 32 * WR::BYTES);
+      aw[j] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
+  auto read_scales = [&](const uint8_t* st, int(&ax)[TX], int(&aw)[TW]) {
+#pragma unroll
+    for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<const int*>(st + xsa + i * 128) >> (8 * half);
+#pragma unroll
+    for (int j = 0; j < TW; ++j) aw[j] = *reinterpret_cast<const int*>(st + wsa + j * 128) >> (8 * half);
+  };
+  f32x16_t acc[TX][TW] = {};
+#define MX_MMA(U, SX, SW)                                                                                             \
+  _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j) acc[i][j] =            \
+      __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[U][j], fx[U][i], acc[i][j], 4, FX == MX_E4M3 ? 0 : 4, 2 * U, \
+                                                      SW[j], 2 * U, SX[i]);
+
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) issue(s, s);
+  ai4e_conv::wait_vmcnt<(STAGES - 1) * PER_STAGE>();
+  __builtin_amdgcn_s_barrier();
+  read_scales(lds, sx[0], sw[0]);
+  read(lds, 0, fx[0], fw[0]);
+  uint32_t slot = 0;
+  // step kt: its first half's fragments and scales are in registers
+#define MX_STEP(KT, CUR, NXT)                                                                                         \
+  {                                                                                                                   \
+    read(lds + slot * STAGE, 1, fx[1], fw[1]);                                                                        \
+    __builtin_amdgcn_sched_barrier(0); /* the reads go out before the matrix instructions that cover them */          \
+    MX_MMA(0, sx[CUR], sw[CUR])                                                                                       \
+    /* this wave's part of step kt + 1 is there and it has read all of step kt: after the barrier step kt + 1 is */   \
+    /* complete and step kt's slot free */                                                                            \
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * PER_STAGE) : "memory");                        \
+    __builtin_amdgcn_s_barrier();                                                                                     \
+    issue((KT) + STAGES, slot);                                                                                       \
+    slot = slot + 1 == STAGES ? 0 : slot + 1;                                                                         \
+    read_scales(lds + slot * STAGE, sx[NXT], sw[NXT]);                                                                \
+    read(lds + slot * STAGE, 0, fx[0], fw[0]);                                                                        \
+    __builtin_amdgcn_sched_barrier(0);                                                                                \
+    MX_MMA(1, sx[CUR], sw[CUR])                                                                                       \
+  }
+  for (int kt = 0; kt + 1 < nk; kt += 2) {
+    MX_STEP(kt, 0, 1)
+    MX_STEP(kt + 1, 1, 0)
+  }
+  if (nk & 1) MX_STEP(nk - 1, 0, 1)
+  ai4e_conv::wait_vmcnt<0>();
+#undef MX_STEP
+#undef MX_MMA
+
+  typedef typename mx_elem<DT>::type E;
+#pragma unroll
+  for (int i = 0; i < TX; ++i) {
+    const int row = x0 + xrow + i * 32;
+    if (row >= m) continue;
+    E* yr = y + static_cast<long>(row) * n;
+#pragma unroll
+    for (int j = 0; j < TW; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int col = w0 + (ww * TW + j) * 32 + 8 * q + 4 * half;
+        struct __attribute__((packed, aligned(sizeof(E)))) Four { E v[4]; } o;
+        if (col + 4 <= n) {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) o.v[p] = mx_elem<DT>::from(acc[i][j][4 * q + p] + (bias ? bias[col + p] : 0.f));
+          *reinterpret_cast<Four*>(yr + col) = o;
+        } else {
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+            if (col + p < n) yr[col + p] = mx_elem<DT>::from(acc[i][j][4 * q + p] + (bias ? bias[col + p] : 0.f));
+        }
+      }
+  }
+}
+
+template <int FX, int DT, int WX, int WW, int TX, int TW, int STAGES>
+int launch_tile(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
+                hipStream_t s) {
+  constexpr int BX = WX * TX * 32, BW = WW * TW * 32;
+  constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES + (BX + BW) * 4);
+  const int tx = ai4e_cdiv(m, BX), tw = ai4e_cdiv(n, BW);
+  auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES>;
+  static const hipError_t ready =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  if (ready != hipSuccess) return AI4E_ELAUNCH;
+  hipLaunchKernelGGL(kernel, dim3(tx * tw), dim3(WX * WW * 64), LDS, s, static_cast<const uint8_t*>(x),
+                     static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(ws),
+                     static_cast<const float*>(bias), m, n, kp, tx, tw, static_cast<typename mx_elem<DT>::type*>(y));
+  return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
 }
 
 }  // namespace
@@ -63,19 +237,20 @@ __global__ __launch_bounds__(256) void mx_linear_kernel(const uint8_t* __restric
 AI4E_API int ai4e_mx_linear(const void* x, const void* xs, int fx, const void* w, const void* ws, const void* bias,
                             int m, int n, int kp, void* y, int dt, hipStream_t s) {
   if (!x || !xs || !w || !ws || !y || m < 0 || n <= 0 || kp <= 0 || kp % MX_ALIGN || fx < 0 || fx > 1 || dt < 0 || dt > 2 ||
-      n > (1 << 30) || m > (1 << 30) || static_cast<long>((m + 31) / 32) * ((n + 31) / 32) > (1L << 25))
+      kp > (1 << 23) || n > (1 << 30) || m > (1 << 30) || static_cast<long>(ai4e_cdiv(m, 128)) * ai4e_cdiv(n, 128) > (1L << 22))
     return AI4E_EINVAL;
   if (m == 0) return AI4E_OK;
-  const dim3 grid(ai4e_cdiv(static_cast<long>((m + 31) / 32) * ((n + 31) / 32), 4)), block(256);
-#define GO(FX, DT)                                                                                                     \
-  hipLaunchKernelGGL((mx_linear_kernel<FX, DT>), grid, block, 0, s, static_cast<const uint8_t*>(x),                    \
-                     static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(ws), \
-                     static_cast<const float*>(bias), m, n, kp, static_cast<mx_elem<DT>::type*>(y))
+#define GO(FX, DT)                                                                                             \
+  return static_cast<long>(ai4e_cdiv(m, 256)) * ai4e_cdiv(n, 256) >= 128                                       \
+             ? launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(x, xs, w, ws, bias, m, n, kp, y, s)                          \
+             : launch_tile<FX, DT, 2, 2, 2, 2, 3>(x, xs, w, ws, bias, m, n, kp, y, s)
   if (fx == MX_E4M3) {
-    if (dt == MX_BF16) GO(MX_E4M3, MX_BF16); else if (dt == MX_F16) GO(MX_E4M3, MX_F16); else GO(MX_E4M3, MX_F32);
-  } else {
-    if (dt == MX_BF16) GO(MX_E2M1, MX_BF16); else if (dt == MX_F16) GO(MX_E2M1, MX_F16); else GO(MX_E2M1, MX_F32);
+    if (dt == MX_BF16) GO(MX_E4M3, MX_BF16);
+    if (dt == MX_F16) GO(MX_E4M3, MX_F16);
+    GO(MX_E4M3, MX_F32);
   }
+  if (dt == MX_BF16) GO(MX_E2M1, MX_BF16);
+  if (dt == MX_F16) GO(MX_E2M1, MX_F16);
+  GO(MX_E2M1, MX_F32);
 #undef GO
-  return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
 }
