@@ -9,6 +9,8 @@
 //   of D it holds column l & 31 (a row of x), rows 8 (i >> 2) + 4 (l >> 5) + (i & 3), i = 0..15 (rows of w)
 // Operands of registers alone run at 4.4 PFLOP/s with e4m3 on one side and 8.0 with e2m1 on both, whose 32 x 32 x 64
 // form is twice as fast as the 16 x 16 x 128 one; hence the large tiles are made of it.
+#include <type_traits>
+
 #include "conv_common.h"
 #include "mx.h"
 
@@ -17,7 +19,7 @@ namespace {
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
-// 16 B (4 B) per lane from base + off to LDS at (wave-uniform lds + 16 (4) * lane); completion is counted by vmcnt.
+// 16 B per lane from base + off to LDS at (wave-uniform lds + 16 * lane); completion is counted by vmcnt.
 // M0 is put back: the compiler reserves it.
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
   uint32_t keep;
@@ -31,17 +33,21 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t l
       : "v"(off), "s"(base), "s"(lds)
       : "memory");
 }
-__device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t lds) {
-  uint32_t keep;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dword %1, %2\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(keep)
-      : "v"(off), "s"(base), "s"(lds)
-      : "memory");
+
+// four consecutive outputs of a row, those below n
+template <int DT>
+__device__ __forceinline__ void store4(typename mx_elem<DT>::type* yr, int col, int n, const float* bias, const f32x4_t& v) {
+  typedef typename mx_elem<DT>::type E;
+  struct __attribute__((packed, aligned(sizeof(E)))) Four { E v[4]; } o;
+  if (col + 4 <= n) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) o.v[p] = mx_elem<DT>::from(v[p] + (bias ? bias[col + p] : 0.f));
+    *reinterpret_cast<Four*>(yr + col) = o;
+  } else {
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      if (col + p < n) yr[col + p] = mx_elem<DT>::from(v[p] + (bias ? bias[col + p] : 0.f));
+  }
 }
 
 // Rows of a tile in LDS, 128 elements each: 128 B (e4m3) or 64 B (e2m1). A DMA writes 1024 consecutive bytes, 8 or 16
@@ -64,12 +70,12 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   constexpr int NW = WX * WW, BX = WX * TX * 32, BW = WW * TW * 32;
   typedef TileRow<FX> XR;
   typedef TileRow<MX_E2M1> WR;
-  constexpr int X_BYTES = BX * XR::BYTES, W_BYTES = BW * WR::BYTES, S_BYTES = (BX + BW) * 4;
-  constexpr int STAGE = X_BYTES + W_BYTES + S_BYTES;
-  constexpr int X_DMA = X_BYTES / 1024 / NW, W_DMA = W_BYTES / 1024 / NW, S_DMA = (BX + BW) / 64;
-  constexpr int PER_STAGE = X_DMA + W_DMA + 1;
-  static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && S_DMA <= NW && BX % 64 == 0 && BW % 64 == 0, "");
-  static_assert(STAGE * STAGES <= 160 * 1024, "");
+  constexpr int X_BYTES = BX * XR::BYTES, W_BYTES = BW * WR::BYTES, S_BYTES = (BX + BW) * 16;
+  constexpr int STAGE = X_BYTES + W_BYTES, SCALES = STAGE * STAGES;
+  constexpr int X_DMA = X_BYTES / 1024 / NW, W_DMA = W_BYTES / 1024 / NW;
+  constexpr int PER_STAGE = X_DMA + W_DMA;
+  static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && S_BYTES == 1024 * NW && BX % 64 == 0, "");
+  static_assert(SCALES + 2 * S_BYTES <= 160 * 1024 && STAGES <= 4, "");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -93,9 +99,8 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     const int row = (wave * W_DMA + j) * WR::PER_DMA + lane / WR::CHUNKS;
     woff[j] = static_cast<uint32_t>(min(row, n - 1 - w0)) * pw + ((lane % WR::CHUNKS) ^ WR::swizzle(row)) * 16;
   }
-  const int sd = wave % S_DMA;  // a wave brings 64 rows' scales
-  const bool s_of_x = sd < BX / 64;
-  const int srow = s_of_x ? min(sd * 64 + lane, m - 1 - x0) : min((sd - BX / 64) * 64 + lane, n - 1 - w0);
+  const bool s_of_x = wave < BX / 64;  // a wave brings 64 rows' scales
+  const int srow = s_of_x ? min(wave * 64 + lane, m - 1 - x0) : min(wave * 64 - BX + lane, n - 1 - w0);
   const uint32_t soff = static_cast<uint32_t>(srow) * ps;
   const uint8_t* xb = x + static_cast<long>(x0) * px;
   const uint8_t* wb = w + static_cast<long>(w0) * pw;
@@ -104,113 +109,111 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   const int nk = kp / MX_ALIGN;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
       (__attribute__((address_space(3))) uint8_t*)lds));
+  // scales come 16 B of a row at a time, for 4 steps: as 4-B pieces they would be as many requests to L2 as the data
+  // (measured: the rate of requests was what bound the kernel). Two slots; the last group ends with the row.
+  auto scales = [&](int g) {
+    dma16(sb + static_cast<long>(min(4 * g, nk - 4)) * 4, soff, lds0 + SCALES + (g & 1) * S_BYTES + wave * 1024);
+  };
   auto issue = [&](int kt, uint32_t slot) {  // past the end the last step is brought again, into a slot nobody reads
     const int k = min(kt, nk - 1);
     const uint32_t base = lds0 + slot * STAGE;
+    if ((kt & 3) == 0) scales(kt / 4);
 #pragma unroll
     for (int j = 0; j < X_DMA; ++j)
       dma16(xb + static_cast<long>(k) * XR::BYTES, xoff[j], base + (wave * X_DMA + j) * 1024);
 #pragma unroll
     for (int j = 0; j < W_DMA; ++j)
       dma16(wb + static_cast<long>(k) * WR::BYTES, woff[j], base + X_BYTES + (wave * W_DMA + j) * 1024);
-    dma4(sb + static_cast<long>(k) * 4, soff, base + X_BYTES + W_BYTES + sd * 256);
   };
 
   const int wx = wave % WX, ww = wave / WX;
   const int r = lane & 31;
   const int xrow = wx * TX * 32 + r, wrow = ww * TW * 32 + r;
-  const int xa = xrow * XR::BYTES + (half ^ XR::swizzle(xrow)) * 16;
-  const int wa = X_BYTES + wrow * WR::BYTES + (half ^ WR::swizzle(wrow)) * 16;
-  const int xsa = X_BYTES + W_BYTES + xrow * 4, wsa = X_BYTES + W_BYTES + (BX + wrow) * 4;
+  const uint32_t xa = xrow * XR::BYTES + (half ^ XR::swizzle(xrow)) * 16;
+  const uint32_t wa = X_BYTES + wrow * WR::BYTES + (half ^ WR::swizzle(wrow)) * 16;
+  const uint32_t sa = r * 16;
 
   i32x8_t fx[2][TX], fw[2][TW];
-  int sx[2][TX], sw[2][TW];
-  // fragments of half step u of a stage; the lane's scale bytes are 2 u + half of its row's four
-  auto read = [&](const uint8_t* st, int u, i32x8_t(&ax)[TX], i32x8_t(&aw)[TW]) {
+  int sx[TX], sw[TW], nx[TX], nw[TW];
+  typedef __attribute__((address_space(3))) const i32x4_t* Lds16;
+  typedef __attribute__((address_space(3))) const int* Lds4;
+  // fragments of half step u of the stage at LDS address st
+  auto read = [&](uint32_t st, int u, i32x8_t(&ax)[TX], i32x8_t(&aw)[TW]) {
+    const uint32_t xc = st + xa, wc = (st + wa) ^ (32 * u);
 #pragma unroll
     for (int i = 0; i < TX; ++i) {
       if constexpr (FX == MX_E4M3) {
-        const i32x4_t a = *reinterpret_cast<const i32x4_t*>(st + (xa ^ (64 * u)) + i * 32 * XR::BYTES);
-        const i32x4_t b = *reinterpret_cast<const i32x4_t*>(st + (xa ^ (64 * u + 32)) + i * 32 * XR::BYTES);
+        const i32x4_t a = *reinterpret_cast<Lds16>((xc ^ (64 * u)) + i * 32 * XR::BYTES);
+        const i32x4_t b = *reinterpret_cast<Lds16>((xc ^ (64 * u + 32)) + i * 32 * XR::BYTES);
         ax[i] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
       } else {
-        const i32x4_t a = *reinterpret_cast<const i32x4_t*>(st + (xa ^ (32 * u)) + i * 32 * XR::BYTES);
+        const i32x4_t a = *reinterpret_cast<Lds16>((xc ^ (32 * u)) + i * 32 * XR::BYTES);
         ax[i] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
       }
     }
 #pragma unroll
     for (int j = 0; j < TW; ++j) {
-      const i32x4_t a = *reinterpret_cast<const i32x4_t*>(st + (wa ^ (32 * u)) + j * 32 * WR::BYTES);
+      const i32x4_t a = *reinterpret_cast<Lds16>(wc + j * 32 * WR::BYTES);
       aw[j] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   };
-  auto read_scales = [&](const uint8_t* st, int(&ax)[TX], int(&aw)[TW]) {
+  // a row's four scale bytes of step kt, shifted so that bytes 0 and 2 are those of this half's blocks
+  auto read_scales = [&](int kt, int(&ax)[TX], int(&aw)[TW]) {
+    const uint32_t st = lds0 + SCALES + ((kt >> 2) & 1) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4 + sa;
 #pragma unroll
-    for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<const int*>(st + xsa + i * 128) >> (8 * half);
+    for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<Lds4>(st + wx * TX * 512 + i * 512);
 #pragma unroll
-    for (int j = 0; j < TW; ++j) aw[j] = *reinterpret_cast<const int*>(st + wsa + j * 128) >> (8 * half);
+    for (int j = 0; j < TW; ++j) aw[j] = *reinterpret_cast<Lds4>(st + BX * 16 + ww * TW * 512 + j * 512);
+  };
+  auto shift_scales = [&]() {
+#pragma unroll
+    for (int i = 0; i < TX; ++i) sx[i] = nx[i] >> (8 * half);
+#pragma unroll
+    for (int j = 0; j < TW; ++j) sw[j] = nw[j] >> (8 * half);
   };
   f32x16_t acc[TX][TW] = {};
-#define MX_MMA(U, SX, SW)                                                                                             \
+#define MX_MMA(U)                                                                                                     \
   _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j) acc[i][j] =            \
       __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[U][j], fx[U][i], acc[i][j], 4, FX == MX_E4M3 ? 0 : 4, 2 * U, \
-                                                      SW[j], 2 * U, SX[i]);
+                                                      sw[j], 2 * U, sx[i]);
 
 #pragma unroll
   for (int s = 0; s < STAGES; ++s) issue(s, s);
   ai4e_conv::wait_vmcnt<(STAGES - 1) * PER_STAGE>();
   __builtin_amdgcn_s_barrier();
-  read_scales(lds, sx[0], sw[0]);
-  read(lds, 0, fx[0], fw[0]);
+  read_scales(0, nx, nw);
+  read(lds0, 0, fx[0], fw[0]);
   uint32_t slot = 0;
-  // step kt: its first half's fragments and scales are in registers
-#define MX_STEP(KT, CUR, NXT)                                                                                         \
-  {                                                                                                                   \
-    read(lds + slot * STAGE, 1, fx[1], fw[1]);                                                                        \
-    __builtin_amdgcn_sched_barrier(0); /* the reads go out before the matrix instructions that cover them */          \
-    MX_MMA(0, sx[CUR], sw[CUR])                                                                                       \
-    /* this wave's part of step kt + 1 is there and it has read all of step kt: after the barrier step kt + 1 is */   \
-    /* complete and step kt's slot free */                                                                            \
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * PER_STAGE) : "memory");                        \
-    __builtin_amdgcn_s_barrier();                                                                                     \
-    issue((KT) + STAGES, slot);                                                                                       \
-    slot = slot + 1 == STAGES ? 0 : slot + 1;                                                                         \
-    read_scales(lds + slot * STAGE, sx[NXT], sw[NXT]);                                                                \
-    read(lds + slot * STAGE, 0, fx[0], fw[0]);                                                                        \
-    __builtin_amdgcn_sched_barrier(0);                                                                                \
-    MX_MMA(1, sx[CUR], sw[CUR])                                                                                       \
+  // at step kt its first half's fragments and its scales are in registers
+  for (int kt = 0; kt < nk; ++kt) {
+    shift_scales();
+    read(lds0 + slot * STAGE, 1, fx[1], fw[1]);
+    __builtin_amdgcn_sched_barrier(0);  // the reads go out before the matrix instructions that cover them
+    MX_MMA(0)
+    // this wave's part of step kt + 1 is there and it has read all of step kt: after the barrier step kt + 1 is
+    // complete and step kt's slot free
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * PER_STAGE) : "memory");
+    __builtin_amdgcn_s_barrier();
+    issue(kt + STAGES, slot);
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
+    read_scales(min(kt + 1, nk - 1), nx, nw);
+    read(lds0 + slot * STAGE, 0, fx[0], fw[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    MX_MMA(1)
   }
-  for (int kt = 0; kt + 1 < nk; kt += 2) {
-    MX_STEP(kt, 0, 1)
-    MX_STEP(kt + 1, 1, 0)
-  }
-  if (nk & 1) MX_STEP(nk - 1, 0, 1)
   ai4e_conv::wait_vmcnt<0>();
-#undef MX_STEP
 #undef MX_MMA
 
-  typedef typename mx_elem<DT>::type E;
 #pragma unroll
   for (int i = 0; i < TX; ++i) {
     const int row = x0 + xrow + i * 32;
     if (row >= m) continue;
-    E* yr = y + static_cast<long>(row) * n;
 #pragma unroll
     for (int j = 0; j < TW; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = w0 + (ww * TW + j) * 32 + 8 * q + 4 * half;
-        struct __attribute__((packed, aligned(sizeof(E)))) Four { E v[4]; } o;
-        if (col + 4 <= n) {
-#pragma unroll
-          for (int p = 0; p < 4; ++p) o.v[p] = mx_elem<DT>::from(acc[i][j][4 * q + p] + (bias ? bias[col + p] : 0.f));
-          *reinterpret_cast<Four*>(yr + col) = o;
-        } else {
-#pragma unroll
-          for (int p = 0; p < 4; ++p)
-            if (col + p < n) yr[col + p] = mx_elem<DT>::from(acc[i][j][4 * q + p] + (bias ? bias[col + p] : 0.f));
-        }
-      }
+      for (int q = 0; q < 4; ++q)
+        store4<DT>(y + static_cast<long>(row) * n, w0 + (ww * TW + j) * 32 + 8 * q + 4 * half, n, bias,
+                   f32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
   }
 }
 
@@ -218,7 +221,7 @@ template <int FX, int DT, int WX, int WW, int TX, int TW, int STAGES>
 int launch_tile(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
                 hipStream_t s) {
   constexpr int BX = WX * TX * 32, BW = WW * TW * 32;
-  constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES + (BX + BW) * 4);
+  constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES) + 2 * (BX + BW) * 16;
   const int tx = ai4e_cdiv(m, BX), tw = ai4e_cdiv(n, BW);
   auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES>;
   static const hipError_t ready =
@@ -228,6 +231,127 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
                      static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(ws),
                      static_cast<const float*>(bias), m, n, kp, tx, tw, static_cast<typename mx_elem<DT>::type*>(y));
   return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
+}
+
+// The slice kernel: 16 MT rows of x by 16 NT rows of w per workgroup, k cut over its 8 waves. Few rows of x leave w's bytes
+// as what it takes, so w goes from memory to registers, each byte once per 16 MT rows of x, in steps of
+// v_mfma_scale_f32_16x16x128: lane l holds row l & 15, k = 32 (l >> 4) .. + 31 of e2m1, 16 (l >> 4) .. + 15 and
+// 64 + 16 (l >> 4) .. + 15 of e4m3, the scale of block l >> 4; of D column l & 15, rows 4 (l >> 4) + i. Four steps' loads go
+// out together, their scales as one 16-B load per row. The waves' sums are added in LDS, always in the same order.
+constexpr int SLICES = 8;
+
+template <int FX, int DT, int MT, int NT>
+__global__ __launch_bounds__(SLICES * 64) void mx_slice_kernel(
+    const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w,
+    const uint8_t* __restrict__ ws, const float* __restrict__ bias, int m, int n, int kp, int tiles_m,
+    typename mx_elem<DT>::type* __restrict__ y) {
+  __shared__ f32x4_t part[SLICES][MT * NT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+  const int t = xcd_remap(blockIdx.x, gridDim.x);  // the row blocks of one w block follow each other: its L2 serves them
+  const int m0 = (t % tiles_m) * 16 * MT, n0 = (t / tiles_m) * 16 * NT;
+  const int nk = kp / MX_ALIGN, k0 = nk * wave / SLICES, k1 = nk * (wave + 1) / SLICES;
+  const long px = FX == MX_E4M3 ? kp : kp / 2, pw = kp / 2, ps = kp / 32;
+  const uint8_t *xr[MT], *xsr[MT], *wr[NT], *wsr[NT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int row = min(m0 + 16 * i + (lane & 15), m - 1);
+    xr[i] = x + row * px + 16 * g;
+    xsr[i] = xs + row * ps;
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int row = min(n0 + 16 * j + (lane & 15), n - 1);
+    wr[j] = w + row * pw + 16 * g;
+    wsr[j] = ws + row * ps;
+  }
+  f32x4_t acc[MT][NT] = {};
+  auto steps = [&](int kt, auto count) {
+    constexpr int S = decltype(count)::value;
+    struct __attribute__((packed, aligned(4))) Scales { int v[S]; };
+    Scales sx[MT], sw[NT];
+    i32x4_t b[NT][S], a0[MT][S], a1[MT][S];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      sw[j] = *reinterpret_cast<const Scales*>(wsr[j] + kt * 4);
+#pragma unroll
+      for (int s = 0; s < S; ++s) b[j][s] = *reinterpret_cast<const i32x4_t*>(wr[j] + (kt + s) * 64l);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      sx[i] = *reinterpret_cast<const Scales*>(xsr[i] + kt * 4);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        a0[i][s] = *reinterpret_cast<const i32x4_t*>(xr[i] + (kt + s) * static_cast<long>(TileRow<FX>::BYTES));
+        if constexpr (FX == MX_E4M3) a1[i][s] = *reinterpret_cast<const i32x4_t*>(xr[i] + (kt + s) * 128l + 64);
+        else a1[i][s] = i32x4_t{};
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              __builtin_shufflevector(b[j][s], i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7),
+              __builtin_shufflevector(a0[i][s], a1[i][s], 0, 1, 2, 3, 4, 5, 6, 7), acc[i][j], 4, FX == MX_E4M3 ? 0 : 4, 0,
+              sw[j].v[s] >> (8 * g), 0, sx[i].v[s] >> (8 * g));
+  };
+  int kt = k0;
+  for (; kt + 4 <= k1; kt += 4) steps(kt, std::integral_constant<int, 4>{});
+  for (; kt < k1; ++kt) steps(kt, std::integral_constant<int, 1>{});
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j) part[wave][i * NT + j][lane] = acc[i][j];
+  __syncthreads();
+  for (int f = wave; f < MT * NT; f += SLICES) {
+    f32x4_t v = part[0][f][lane];
+#pragma unroll
+    for (int p = 1; p < SLICES; ++p) v += part[p][f][lane];
+    const int row = m0 + 16 * (f / NT) + (lane & 15), col = n0 + 16 * (f % NT) + 4 * g;
+    if (row < m) store4<DT>(y + static_cast<long>(row) * n, col, n, bias, v);
+  }
+}
+
+template <int FX, int DT, int MT, int NT>
+int launch_slice(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
+                 hipStream_t s) {
+  const int tm = ai4e_cdiv(m, 16 * MT);
+  hipLaunchKernelGGL((mx_slice_kernel<FX, DT, MT, NT>), dim3(tm * ai4e_cdiv(n, 16 * NT)), dim3(SLICES * 64), 0, s,
+                     static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w),
+                     static_cast<const uint8_t*>(ws), static_cast<const float*>(bias), m, n, kp, tm,
+                     static_cast<typename mx_elem<DT>::type*>(y));
+  return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
+}
+
+template <int FX, int DT>
+int launch(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
+           hipStream_t s) {
+#define ARGS x, xs, w, ws, bias, m, n, kp, y, s
+#ifdef MX_FORCE
+  static const int force = getenv("MX_FORCE") ? atoi(getenv("MX_FORCE")) : 0;
+  if (force == 1) return launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(ARGS);
+  if (force == 2) return launch_tile<FX, DT, 2, 2, 2, 2, 3>(ARGS);
+  if (force == 3) return launch_slice<FX, DT, 1, 1>(ARGS);
+  if (force == 4) return launch_slice<FX, DT, 1, 2>(ARGS);
+  if (force == 5) return launch_slice<FX, DT, 1, 4>(ARGS);
+  if (force == 6) return launch_slice<FX, DT, 2, 1>(ARGS);
+  if (force == 7) return launch_slice<FX, DT, 2, 2>(ARGS);
+  if (force == 8) return launch_slice<FX, DT, 2, 4>(ARGS);
+  if (force == 9) return launch_slice<FX, DT, 4, 1>(ARGS);
+  if (force == 10) return launch_slice<FX, DT, 4, 2>(ARGS);
+#endif
+  if (kp >= 512 && m > 64) {
+    if (static_cast<long>(ai4e_cdiv(m, 256)) * ai4e_cdiv(n, 256) >= 128)
+      return launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(ARGS);
+    if (static_cast<long>(ai4e_cdiv(m, 128)) * ai4e_cdiv(n, 128) >= 64) return launch_tile<FX, DT, 2, 2, 2, 2, 3>(ARGS);
+  }
+  const bool wide = n >= 16384;
+  if (m <= 16) return wide ? launch_slice<FX, DT, 1, 4>(ARGS) : launch_slice<FX, DT, 1, 1>(ARGS);
+  if (m <= 32) return wide ? launch_slice<FX, DT, 2, 4>(ARGS) : launch_slice<FX, DT, 2, 1>(ARGS);
+  return wide ? launch_slice<FX, DT, 4, 2>(ARGS) : launch_slice<FX, DT, 4, 1>(ARGS);
+#undef ARGS
 }
 
 }  // namespace
@@ -240,10 +364,7 @@ AI4E_API int ai4e_mx_linear(const void* x, const void* xs, int fx, const void* w
       kp > (1 << 23) || n > (1 << 30) || m > (1 << 30) || static_cast<long>(ai4e_cdiv(m, 128)) * ai4e_cdiv(n, 128) > (1L << 22))
     return AI4E_EINVAL;
   if (m == 0) return AI4E_OK;
-#define GO(FX, DT)                                                                                             \
-  return static_cast<long>(ai4e_cdiv(m, 256)) * ai4e_cdiv(n, 256) >= 128                                       \
-             ? launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(x, xs, w, ws, bias, m, n, kp, y, s)                          \
-             : launch_tile<FX, DT, 2, 2, 2, 2, 3>(x, xs, w, ws, bias, m, n, kp, y, s)
+#define GO(FX, DT) return launch<FX, DT>(x, xs, w, ws, bias, m, n, kp, y, s)
   if (fx == MX_E4M3) {
     if (dt == MX_BF16) GO(MX_E4M3, MX_BF16);
     if (dt == MX_F16) GO(MX_E4M3, MX_F16);
