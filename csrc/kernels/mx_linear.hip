@@ -75,7 +75,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   constexpr int X_DMA = X_BYTES / 1024 / NW, W_DMA = W_BYTES / 1024 / NW;
   constexpr int PER_STAGE = X_DMA + W_DMA;
   static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && S_BYTES == 1024 * NW && BX % 64 == 0, "");
-  static_assert(SCALES + 2 * S_BYTES <= 160 * 1024 && STAGES <= 4, "");
+  static_assert(SCALES + 2 * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 4, "");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -114,16 +114,14 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   auto scales = [&](int g) {
     dma16(sb + static_cast<long>(min(4 * g, nk - 4)) * 4, soff, lds0 + SCALES + (g & 1) * S_BYTES + wave * 1024);
   };
-  auto issue = [&](int kt, uint32_t slot) {  // past the end the last step is brought again, into a slot nobody reads
+  // piece j of step kt; past the end the last step is brought again, into a slot that nobody reads
+  auto issue = [&](int kt, uint32_t slot, int j) {
     const int k = min(kt, nk - 1);
     const uint32_t base = lds0 + slot * STAGE;
-    if ((kt & 3) == 0) scales(kt / 4);
-#pragma unroll
-    for (int j = 0; j < X_DMA; ++j)
+    if (j < X_DMA)
       dma16(xb + static_cast<long>(k) * XR::BYTES, xoff[j], base + (wave * X_DMA + j) * 1024);
-#pragma unroll
-    for (int j = 0; j < W_DMA; ++j)
-      dma16(wb + static_cast<long>(k) * WR::BYTES, woff[j], base + X_BYTES + (wave * W_DMA + j) * 1024);
+    else
+      dma16(wb + static_cast<long>(k) * WR::BYTES, woff[j - X_DMA], base + X_BYTES + (wave * W_DMA + j - X_DMA) * 1024);
   };
 
   const int wx = wave % WX, ww = wave / WX;
@@ -137,24 +135,21 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   int sx[TX], sw[TW], nx[TX], nw[TW];
   typedef __attribute__((address_space(3))) const i32x4_t* Lds16;
   typedef __attribute__((address_space(3))) const int* Lds4;
-  // fragments of half step u of the stage at LDS address st
-  auto read = [&](uint32_t st, int u, i32x8_t(&ax)[TX], i32x8_t(&aw)[TW]) {
-    const uint32_t xc = st + xa, wc = (st + wa) ^ (32 * u);
-#pragma unroll
-    for (int i = 0; i < TX; ++i) {
-      if constexpr (FX == MX_E4M3) {
-        const i32x4_t a = *reinterpret_cast<Lds16>((xc ^ (64 * u)) + i * 32 * XR::BYTES);
-        const i32x4_t b = *reinterpret_cast<Lds16>((xc ^ (64 * u + 32)) + i * 32 * XR::BYTES);
-        ax[i] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-      } else {
-        const i32x4_t a = *reinterpret_cast<Lds16>((xc ^ (32 * u)) + i * 32 * XR::BYTES);
-        ax[i] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < TW; ++j) {
-      const i32x4_t a = *reinterpret_cast<Lds16>(wc + j * 32 * WR::BYTES);
-      aw[j] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
+  // piece p of the fragments of half step u of the stage at LDS address st: first w's, then x's (two per row of e4m3)
+  constexpr int PIECES = TW + TX * XR::BYTES / 64;
+  auto read = [&](uint32_t st, int u, int p) {
+    if (p < TW) {
+      const i32x4_t a = *reinterpret_cast<Lds16>(((st + wa) ^ (32 * u)) + p * 32 * WR::BYTES);
+      fw[u][p] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else if constexpr (FX == MX_E4M3) {
+      const int i = (p - TW) / 2, hi = (p - TW) & 1;
+      const i32x4_t a = *reinterpret_cast<Lds16>(((st + xa) ^ (64 * u + 32 * hi)) + i * 32 * XR::BYTES);
+      fx[u][i] = hi ? __builtin_shufflevector(fx[u][i], __builtin_shufflevector(a, a, 0, 1, 2, 3, 0, 1, 2, 3), 0, 1, 2, 3, 8, 9, 10, 11)
+                    : __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      const int i = p - TW;
+      const i32x4_t a = *reinterpret_cast<Lds16>(((st + xa) ^ (32 * u)) + i * 32 * XR::BYTES);
+      fx[u][i] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   };
   // a row's four scale bytes of step kt, shifted so that bytes 0 and 2 are those of this half's blocks
@@ -172,34 +167,52 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     for (int j = 0; j < TW; ++j) sw[j] = nw[j] >> (8 * half);
   };
   f32x16_t acc[TX][TW] = {};
-#define MX_MMA(U)                                                                                                     \
-  _Pragma("unroll") for (int i = 0; i < TX; ++i) _Pragma("unroll") for (int j = 0; j < TW; ++j) acc[i][j] =            \
-      __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[U][j], fx[U][i], acc[i][j], 4, FX == MX_E4M3 ? 0 : 4, 2 * U, \
-                                                      sw[j], 2 * U, sx[i]);
+  constexpr int Q = TX * TW;
+#define MX_MMA(U, N)                                                                                           \
+  acc[(N) / TW][(N) % TW] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                   \
+      fw[U][(N) % TW], fx[U][(N) / TW], acc[(N) / TW][(N) % TW], 4, FX == MX_E4M3 ? 0 : 4, 2 * U, sw[(N) % TW], \
+      2 * U, sx[(N) / TW]);
 
 #pragma unroll
-  for (int s = 0; s < STAGES; ++s) issue(s, s);
+  for (int s = 0; s < STAGES; ++s) {
+    if (s == 0) scales(0);
+#pragma unroll
+    for (int j = 0; j < PER_STAGE; ++j) issue(s, s, j);
+  }
   ai4e_conv::wait_vmcnt<(STAGES - 1) * PER_STAGE>();
   __builtin_amdgcn_s_barrier();
   read_scales(0, nx, nw);
-  read(lds0, 0, fx[0], fw[0]);
+#pragma unroll
+  for (int p = 0; p < PIECES; ++p) read(lds0, 0, p);
   uint32_t slot = 0;
-  // at step kt its first half's fragments and its scales are in registers
+  // At step kt its first half's fragments and its scales are in registers. Reads and DMAs go out between the matrix
+  // instructions, which keep their unit busy meanwhile; the order is fixed by scheduling barriers.
   for (int kt = 0; kt < nk; ++kt) {
     shift_scales();
-    read(lds0 + slot * STAGE, 1, fx[1], fw[1]);
-    __builtin_amdgcn_sched_barrier(0);  // the reads go out before the matrix instructions that cover them
-    MX_MMA(0)
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      MX_MMA(0, q)
+#pragma unroll
+      for (int p = 2 * q; p < 2 * q + 2 && p < PIECES; ++p) read(lds0 + slot * STAGE, 1, p);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     // this wave's part of step kt + 1 is there and it has read all of step kt: after the barrier step kt + 1 is
     // complete and step kt's slot free
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * PER_STAGE) : "memory");
     __builtin_amdgcn_s_barrier();
-    issue(kt + STAGES, slot);
+    const uint32_t free = slot;
     slot = slot + 1 == STAGES ? 0 : slot + 1;
-    read_scales(min(kt + 1, nk - 1), nx, nw);
-    read(lds0 + slot * STAGE, 0, fx[0], fw[0]);
-    __builtin_amdgcn_sched_barrier(0);
-    MX_MMA(1)
+    if (((kt + STAGES) & 3) == 0) scales((kt + STAGES) / 4);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      MX_MMA(1, q)
+      if (q == 0) read_scales(min(kt + 1, nk - 1), nx, nw);
+#pragma unroll
+      for (int p = 2 * q; p < 2 * q + 2 && p < PIECES; ++p) read(lds0 + slot * STAGE, 0, p);
+#pragma unroll
+      for (int j = PER_STAGE * q / Q; j < PER_STAGE * (q + 1) / Q; ++j) issue(kt + STAGES, free, j);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
   ai4e_conv::wait_vmcnt<0>();
 #undef MX_MMA
