@@ -18,6 +18,7 @@ namespace {
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef i32x4_t __attribute__((aligned(2))) Chunk16;  // 16 B of outputs: rows of odd n start at any element
 
 // 16 B per lane from base + off to LDS at (wave-uniform lds + 16 * lane); completion is counted by vmcnt.
 // M0 is put back: the compiler reserves it.
@@ -56,7 +57,7 @@ __device__ __forceinline__ void store4(typename mx_elem<DT>::type* yr, int col, 
 template <int FMT>
 struct TileRow {
   static constexpr int BYTES = FMT == MX_E4M3 ? 128 : 64, CHUNKS = BYTES / 16, PER_DMA = 1024 / BYTES;
-  static __device__ __forceinline__ int swizzle(int row) { return FMT == MX_E4M3 ? row & 7 : ai4e_conv::swz(row); }
+  static __device__ __forceinline__ int swizzle(int row) { return FMT == MX_E4M3 ? (row >> 1) & 7 : ai4e_conv::swz(row); }
 };
 
 // The tile kernel: BX x BW outputs per workgroup, WX x WW waves of TX x TW fragments of 32 x 32. Steps of 128 along k go
@@ -74,7 +75,8 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   constexpr int STAGE = X_BYTES + W_BYTES, SCALES = STAGE * STAGES;
   constexpr int X_DMA = X_BYTES / 1024 / NW, W_DMA = W_BYTES / 1024 / NW;
   constexpr int PER_STAGE = X_DMA + W_DMA;
-  static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && S_BYTES == 1024 * NW && BX % 64 == 0, "");
+  constexpr int S_ALL = S_BYTES / 1024, S_DMA = (S_ALL + NW - 1) / NW;
+  static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && S_BYTES % 1024 == 0 && BX % 64 == 0, "");
   static_assert(SCALES + 2 * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 4, "");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
@@ -99,12 +101,16 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     const int row = (wave * W_DMA + j) * WR::PER_DMA + lane / WR::CHUNKS;
     woff[j] = static_cast<uint32_t>(min(row, n - 1 - w0)) * pw + ((lane % WR::CHUNKS) ^ WR::swizzle(row)) * 16;
   }
-  const bool s_of_x = wave < BX / 64;  // a wave brings 64 rows' scales
-  const int srow = s_of_x ? min(wave * 64 + lane, m - 1 - x0) : min(wave * 64 - BX + lane, n - 1 - w0);
-  const uint32_t soff = static_cast<uint32_t>(srow) * ps;
+  uint32_t soff[S_DMA];  // a DMA brings the scales of 64 rows, first x's, then w's; the odd ones out bring some twice
+#pragma unroll
+  for (int j = 0; j < S_DMA; ++j) {
+    const int p = (wave + j * NW) % S_ALL;
+    soff[j] = static_cast<uint32_t>(p < BX / 64 ? min(p * 64 + lane, m - 1 - x0) : min(p * 64 - BX + lane, n - 1 - w0)) * ps;
+  }
   const uint8_t* xb = x + static_cast<long>(x0) * px;
   const uint8_t* wb = w + static_cast<long>(w0) * pw;
-  const uint8_t* sb = s_of_x ? xs + static_cast<long>(x0) * ps : ws + static_cast<long>(w0) * ps;
+  const uint8_t* xsb = xs + static_cast<long>(x0) * ps;
+  const uint8_t* wsb = ws + static_cast<long>(w0) * ps;
 
   const int nk = kp / MX_ALIGN;
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
@@ -112,7 +118,12 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   // scales come 16 B of a row at a time, for 4 steps: as 4-B pieces they would be as many requests to L2 as the data
   // (measured: the rate of requests was what bound the kernel). Two slots; the last group ends with the row.
   auto scales = [&](int g) {
-    dma16(sb + static_cast<long>(min(4 * g, nk - 4)) * 4, soff, lds0 + SCALES + (g & 1) * S_BYTES + wave * 1024);
+#pragma unroll
+    for (int j = 0; j < S_DMA; ++j) {
+      const int p = (wave + j * NW) % S_ALL;
+      dma16((p < BX / 64 ? xsb : wsb) + static_cast<long>(min(4 * g, nk - 4)) * 4, soff[j],
+            lds0 + SCALES + (g & 1) * S_BYTES + p * 1024);
+    }
   };
   // piece j of step kt; past the end the last step is brought again, into a slot that nobody reads
   auto issue = [&](int kt, uint32_t slot, int j) {
@@ -217,16 +228,51 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   ai4e_conv::wait_vmcnt<0>();
 #undef MX_MMA
 
+  // The wave's outputs go through its own part of the idle ring, 32 rows at a time, so that stores fill whole lines:
+  // straight from the accumulators they are 16-B pieces of 32 rows, whose requests took L2 longer than the data does
+  // (4096 x 16384 x 8192: 55 of 414 us).
+  __builtin_amdgcn_s_barrier();  // every wave has read its last fragments, every DMA has landed
+  typedef typename mx_elem<DT>::type E;
+  constexpr int COLS = TW * 32, CHUNK = 16 / sizeof(E), CHUNKS = COLS / CHUNK;  // 16-B chunks of a row of outputs
+  static_assert(NW * 32 * COLS * sizeof(E) <= SCALES, "");
+  uint8_t* mine = lds + wave * 32 * COLS * sizeof(E);
+  const int c0 = w0 + ww * COLS;
 #pragma unroll
   for (int i = 0; i < TX; ++i) {
-    const int row = x0 + xrow + i * 32;
-    if (row >= m) continue;
 #pragma unroll
     for (int j = 0; j < TW; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        store4<DT>(y + static_cast<long>(row) * n, w0 + (ww * TW + j) * 32 + 8 * q + 4 * half, n, bias,
-                   f32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+      for (int q = 0; q < 4; ++q) {
+        const int col = j * 32 + 8 * q + 4 * half;
+        typedef int Four __attribute__((ext_vector_type(sizeof(E))));  // 4 outputs
+        struct { E v[4]; } o;
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+          o.v[p] = mx_elem<DT>::from(acc[i][j][4 * q + p] + (bias && c0 + col + p < n ? bias[c0 + col + p] : 0.f));
+        const int chunk = (col / CHUNK) ^ (r & (CHUNKS - 1));
+        *reinterpret_cast<Four*>(mine + (r * CHUNKS + chunk) * 16 + col % CHUNK * sizeof(E)) = __builtin_bit_cast(Four, o);
+      }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int it = 0; it < 32 * CHUNKS / 64; ++it) {
+      const int rr = (it * 64 + lane) / CHUNKS, ch = (it * 64 + lane) % CHUNKS;
+      const int row = x0 + (wx * TX + i) * 32 + rr, col = c0 + ch * CHUNK;
+      struct Chunk { E v[CHUNK]; };
+      const Chunk o = __builtin_bit_cast(
+          Chunk, *reinterpret_cast<const i32x4_t*>(mine + (rr * CHUNKS + (ch ^ (rr & (CHUNKS - 1)))) * 16));
+      if (row < m) {
+        E* to = y + static_cast<long>(row) * n + col;
+        if (col + CHUNK <= n) {
+          // past L2: the outputs would push x and w out of it
+          __builtin_nontemporal_store(__builtin_bit_cast(Chunk16, o), reinterpret_cast<Chunk16*>(to));
+        } else {
+#pragma unroll
+          for (int p = 0; p < CHUNK; ++p)
+            if (col + p < n) to[p] = o.v[p];
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
