@@ -178,7 +178,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     for (int j = 0; j < TW; ++j) sw[j] = nw[j] >> (8 * half);
   };
   f32x16_t acc[TX][TW] = {};
-  constexpr int Q = TX * TW;
+  constexpr int Q = TX * TW, READS = PIECES <= 2 * Q ? 2 : (PIECES + Q - 1) / Q;  // pieces read after each instruction
 #define MX_MMA(U, N)                                                                                           \
   acc[(N) / TW][(N) % TW] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(                                   \
       fw[U][(N) % TW], fx[U][(N) / TW], acc[(N) / TW][(N) % TW], 4, FX == MX_E4M3 ? 0 : 4, 2 * U, sw[(N) % TW], \
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     for (int q = 0; q < Q; ++q) {
       MX_MMA(0, q)
 #pragma unroll
-      for (int p = 2 * q; p < 2 * q + 2 && p < PIECES; ++p) read(lds0 + slot * STAGE, 1, p);
+      for (int p = READS * q; p < READS * (q + 1) && p < PIECES; ++p) read(lds0 + slot * STAGE, 1, p);
       __builtin_amdgcn_sched_barrier(0);
     }
     // this wave's part of step kt + 1 is there and it has read all of step kt: after the barrier step kt + 1 is
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
       MX_MMA(1, q)
       if (q == 0) read_scales(min(kt + 1, nk - 1), nx, nw);
 #pragma unroll
-      for (int p = 2 * q; p < 2 * q + 2 && p < PIECES; ++p) read(lds0 + slot * STAGE, 0, p);
+      for (int p = READS * q; p < READS * (q + 1) && p < PIECES; ++p) read(lds0 + slot * STAGE, 0, p);
 #pragma unroll
       for (int j = PER_STAGE * q / Q; j < PER_STAGE * (q + 1) / Q; ++j) issue(kt + STAGES, free, j);
       __builtin_amdgcn_sched_barrier(0);
@@ -292,8 +292,8 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
   return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
 }
 
-// The slice kernel: 16 MT rows of x by 16 NT rows of w per workgroup, k cut over its 8 waves. Few rows of x leave w's bytes
-// as what it takes, so w goes from memory to registers, each byte once per 16 MT rows of x, in steps of
+// The slice kernel: 16 MT rows of x by 16 NT rows of w per workgroup, k cut over its 8 waves: for outputs too few to give
+// every CU a tile, where latency counts. Operands go from memory to registers, in steps of
 // v_mfma_scale_f32_16x16x128: lane l holds row l & 15, k = 32 (l >> 4) .. + 31 of e2m1, 16 (l >> 4) .. + 15 and
 // 64 + 16 (l >> 4) .. + 15 of e4m3, the scale of block l >> 4; of D column l & 15, rows 4 (l >> 4) + i. Four steps' loads go
 // out together, their scales as one 16-B load per row. The waves' sums are added in LDS, always in the same order.
@@ -384,32 +384,32 @@ int launch_slice(const void* x, const void* xs, const void* w, const void* ws, c
   return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
 }
 
+// Which kernel: the largest tile that still gives most of the 256 CUs one, since a larger tile moves fewer bytes per
+// product; where even 64 x 64 does not, slices of k, the smallest that need one round of workgroups. Measured at the
+// borders (us, e4m3, cold weights; the larger of each pair first):
+//   256 x 256 / 128 x 128   1024 x 8192 x 8192 (128 / 512 tiles) 77.7 / 61.8    4096 x 4096 x 4096 (256 / 1024) 55 / 70
+//   128 x 128 / 64 x 128    512 x 4096 x 4096 (128 / 256 tiles) 17.6 / 12.5     512 x 8192 x 8192 (256 / 512) 38.5 / 45.0
+//   64 x 128 / 64 x 64      256 x 4096 x 4096 (128 / 256 tiles) 12.1 / 11.1     256 x 8192 x 8192 (256 / 512) 26.4 / 33.0
+//   few rows, a large w: 16 x 32768 x 8192 128 x 128 42.0, 64 x 128 36.7, slices (1, 4) 38.1
+//   64 x 64 / slices        128 x 4096 x 4096 10.8 / 11.6 (2, 4)   64 x 4096 x 4096 10.7 / 9.0 (2, 2)   16 x 4096 x 4096 5.9 (1, 1)
 template <int FX, int DT>
 int launch(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
            hipStream_t s) {
 #define ARGS x, xs, w, ws, bias, m, n, kp, y, s
-#ifdef MX_FORCE
-  static const int force = getenv("MX_FORCE") ? atoi(getenv("MX_FORCE")) : 0;
-  if (force == 1) return launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(ARGS);
-  if (force == 2) return launch_tile<FX, DT, 2, 2, 2, 2, 3>(ARGS);
-  if (force == 3) return launch_slice<FX, DT, 1, 1>(ARGS);
-  if (force == 4) return launch_slice<FX, DT, 1, 2>(ARGS);
-  if (force == 5) return launch_slice<FX, DT, 1, 4>(ARGS);
-  if (force == 6) return launch_slice<FX, DT, 2, 1>(ARGS);
-  if (force == 7) return launch_slice<FX, DT, 2, 2>(ARGS);
-  if (force == 8) return launch_slice<FX, DT, 2, 4>(ARGS);
-  if (force == 9) return launch_slice<FX, DT, 4, 1>(ARGS);
-  if (force == 10) return launch_slice<FX, DT, 4, 2>(ARGS);
-#endif
-  if (kp >= 512 && m > 64) {
-    if (static_cast<long>(ai4e_cdiv(m, 256)) * ai4e_cdiv(n, 256) >= 128)
+  const auto blocks = [&](int bm, int bn) { return static_cast<long>(ai4e_cdiv(m, bm)) * ai4e_cdiv(n, bn); };
+  constexpr long FILL = 192, ROUND = 320;
+  if (kp >= 512) {  // the tiles' scales come four steps of 128 at a time
+    if (m > 128 && blocks(256, 256) >= FILL)
       return launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(ARGS);
-    if (static_cast<long>(ai4e_cdiv(m, 128)) * ai4e_cdiv(n, 128) >= 64) return launch_tile<FX, DT, 2, 2, 2, 2, 3>(ARGS);
+    if (m > 64 && blocks(128, 128) >= FILL)
+      return launch_tile<FX, DT, 2, 2, 2, 2, FX == MX_E4M3 ? 3 : 4>(ARGS);
+    if (blocks(64, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 2, 4>(ARGS);
   }
-  const bool wide = n >= 16384;
-  if (m <= 16) return wide ? launch_slice<FX, DT, 1, 4>(ARGS) : launch_slice<FX, DT, 1, 1>(ARGS);
-  if (m <= 32) return wide ? launch_slice<FX, DT, 2, 4>(ARGS) : launch_slice<FX, DT, 2, 1>(ARGS);
-  return wide ? launch_slice<FX, DT, 4, 2>(ARGS) : launch_slice<FX, DT, 4, 1>(ARGS);
+  if (blocks(16, 16) <= ROUND) return launch_slice<FX, DT, 1, 1>(ARGS);
+  if (blocks(16, 32) <= ROUND) return launch_slice<FX, DT, 1, 2>(ARGS);
+  if (m <= 16) return launch_slice<FX, DT, 1, 4>(ARGS);
+  if (blocks(32, 32) <= ROUND) return launch_slice<FX, DT, 2, 2>(ARGS);
+  return kp >= 512 ? launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS) : launch_slice<FX, DT, 2, 4>(ARGS);
 #undef ARGS
 }
 

@@ -115,6 +115,15 @@ def test_linear_large(m, n, k, fmt):
     check_linear(m, n, k, fmt, torch.bfloat16, bias=True, seed=m)
 
 
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", torch.bfloat16), ("e4m3", torch.float16), ("e2m1", torch.bfloat16),
+                                       ("e2m1", torch.float32)])
+@pytest.mark.parametrize("m,n,k", [(70, 12500, 1000), (1600, 2001, 640), (3500, 3699, 520), (2500, 300, 200),
+                                   (3300, 4100, 1664)])
+def test_linear_every_tile(m, n, k, fmt, dtype):
+    """64 x 128, 128 x 128 and 256 x 256 tiles, slices of many rows, odd counts of steps."""
+    check_linear(m, n, k, fmt, dtype, bias=True, seed=m)
+
+
 @pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
 @pytest.mark.parametrize("m", [1, 16, 40, 200, 600])
 def test_linear_not_finite_blocks_stay_in_their_row(m, fmt):
