@@ -78,8 +78,7 @@ _SIGS = {
     "ai4e_mx_dequantize": [_vp, _vp, _c_long, _c_int, _c_int, _c_int, _vp, _vp],
     "ai4e_mx_linear": [_vp, _vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp],
     "ai4e_rms_norm_mx8": [_vp, _c_long, _vp, _c_long, _vp, _c_float, _c_long, _c_int, _c_int, _vp, _vp, _vp, _vp],
-    "ai4e_label_logprobs_ws": [_c_long, _c_int, _c_int],
-    "ai4e_label_logprobs": [_vp, _c_long, _c_long, _c_int, _c_int, _vp, _c_int, _c_int, _c_int] + [_vp] * 6,
+    "ai4e_label_logprobs": [_vp, _c_long, _c_long, _c_int, _c_int, _vp, _c_int, _c_int, _c_int] + [_vp] * 5,
     "ai4e_crumbs_alloc": [_c_int, _vp, _vp],
     "ai4e_crumb": [_vp, _c_int, _vp],
 }

@@ -70,11 +70,9 @@ def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, 
     rows = x.shape[0]
     if rows:
         labels = None if labels is None else labels.contiguous()
-        words = _ext.call_int("ai4e_label_logprobs_ws", rows, c, k)
-        ws = torch.empty(words, device=dev, dtype=torch.float32) if words else None
         _ext.call_on(dev, "ai4e_label_logprobs", x.data_ptr(), max(x.stride(0), c), rows, c, mx.DTYPE_CODE[x.dtype],
                      _ext.ptr(labels) if n_labels else None, int(n_labels > 0 and labels.dtype == torch.int64), n_labels, k,
-                     _ext.ptr(logp), entropy.data_ptr(), top_idx.data_ptr(), top_logp.data_ptr(), _ext.ptr(ws))
+                     _ext.ptr(logp), entropy.data_ptr(), top_idx.data_ptr(), top_logp.data_ptr())
     return LabelLogprobs(logp, entropy, top_idx, top_logp)
 
 

@@ -5,21 +5,20 @@
 //   logp(j) = x_j - m - log s               entropy = log s - t / s
 //
 // One pass: a lane keeps (m, s, t) of the elements it has seen and rescales s and t when its maximum grows, so a logit
-// is read once and memory bounds the kernel. The differences x - m are taken before the change to base 2: masks of the
-// type's lowest value stay finite, and -inf gives e = 0.
+// is read once and memory bounds the kernel on large inputs, the row's phases on small ones. The differences x - m are
+// taken before the change to base 2: masks of the type's lowest value stay finite, and -inf gives e = 0.
 //
-// The k best come out of the same pass. A lane also keeps its best chunk (8 consecutive logits; the first one with the
-// lane's maximum). The k-th largest of the lanes' (maximum, chunk) pairs bounds the k-th best logit from below, so only
-// the k lanes at or above it hold candidates: their chunks are read again (from cache), what reaches the bound is put
-// into LDS, and each candidate's rank is the number of candidates before it. Ties go to the lower class. If more
-// candidates come than LDS has room for (their order on the row is adverse), k rounds over the row find one each.
-//
-// A row of few, long rows is split over `splits` workgroups, whose (m, s, t) and k best are joined by a second launch.
+// The k best come out of the same pass (logprobs_kernel). A lane also keeps its best chunk (8 consecutive logits; the
+// first one with the lane's maximum). The k-th largest of 256 groups' (maximum, chunk) pairs bounds the k-th best logit
+// from below, so only the k groups at or above it hold candidates: their chunks are read again (from cache), what reaches
+// the bound is put into LDS, and each candidate's rank is the number of candidates before it. Ties go to the lower class.
+// If more candidates come than LDS has room for (their order on the row is adverse), k rounds over the row find one each.
+// Short rows with few alternatives stay in one wave's registers (logprobs_wave_kernel).
 #include "mx.h"
 
 namespace {
 
-constexpr int T = 256, WAVES = T / 64, KMAX = 64, CAP = 1024, SPLITS_MAX = 64;
+constexpr int KMAX = 64, CAP = 1024, GROUPS = 256;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LOWEST = -3.402823466e38f;
 constexpr float FAR = -200.f;  // e^FAR is 0 in 32 bits; keeps 0 * (x - m) from being 0 * -inf
@@ -30,20 +29,45 @@ struct Stat {
 
 __device__ __forceinline__ float exp_(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 
-// both parts' sums, relative to the larger maximum
-__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
-  const float m = fmaxf(a.m, b.m);
-  const float da = a.m - m, db = b.m - m, fa = exp_(da), fb = exp_(db);
-  return {m, a.s * fa + b.s * fb, fa * (a.t + fmaxf(da, FAR) * a.s) + fb * (b.t + fmaxf(db, FAR) * b.s)};
+// v's sums relative to a maximum m >= v.m
+__device__ __forceinline__ Stat rescaled(const Stat& v, float m) {
+  const float d = v.m - m, f = exp_(d);
+  return {m, v.s * f, f * (v.t + fmaxf(d, FAR) * v.s)};
 }
 
-__device__ __forceinline__ Stat wave_join(Stat v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const Stat w = {__shfl_xor(v.m, o, 64), __shfl_xor(v.s, o, 64), __shfl_xor(v.t, o, 64)};
-    v = join(v, w);
-  }
-  return v;
+// lane i's value from lane i ^ 1, i ^ 2, 7 - i of 8, 15 - i of 16: four steps that join 16 lanes
+template <int STEP>
+__device__ __forceinline__ int dpp(int v) {
+  constexpr int CTRL[4] = {0xB1, 0x4E, 0x141, 0x140};
+  return __builtin_amdgcn_mov_dpp(v, CTRL[STEP], 0xF, 0xF, true);
+}
+template <int STEP>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(dpp<STEP>(__float_as_int(v)));
+}
+template <typename V, typename F>
+__device__ __forceinline__ V wave_all(V v, F op) {
+  v = op(v, dpp<0>(v));
+  v = op(v, dpp<1>(v));
+  v = op(v, dpp<2>(v));
+  v = op(v, dpp<3>(v));
+  const int b = __builtin_bit_cast(int, v);
+  const V v0 = __builtin_bit_cast(V, __builtin_amdgcn_readlane(b, 0)), v1 = __builtin_bit_cast(V, __builtin_amdgcn_readlane(b, 16));
+  const V v2 = __builtin_bit_cast(V, __builtin_amdgcn_readlane(b, 32)), v3 = __builtin_bit_cast(V, __builtin_amdgcn_readlane(b, 48));
+  return op(op(v0, v1), op(v2, v3));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  return wave_all(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ int wave_min(int v) {
+  return wave_all(v, [](int a, int b) { return min(a, b); });
+}
+__device__ __forceinline__ Stat wave_join(const Stat& v) {
+  const Stat r = rescaled(v, wave_max(v.m));
+  return {r.m, wave_sum(r.s), wave_sum(r.t)};
 }
 
 // larger value first, then the lower class
@@ -66,205 +90,18 @@ __device__ __forceinline__ void load_chunk(const typename mx_elem<DT>::type* x, 
     mx_load8_tail<DT>(x + c, n - c, -INFINITY, f);
 }
 
-struct Shared {
-  Stat stat[WAVES];
-  uint32_t key[T];     // each lane's maximum (ordered; 0: it has seen nothing over -inf) and chunk
-  int chunk[T];
-  uint32_t bound;      // the k-th largest of the keys, and among equal ones the last chunk that counts
-  int bound_chunk;
-  int lanes[KMAX];     // lanes at or over the bound
-  int n_lanes, n_cand;
-  float value[CAP];
-  int index[CAP];
-  float round_value[WAVES];
-  int round_index[WAVES];
-};
-
-// the k-th largest (key, lower chunk first) of the T lanes, by the first wave: the key bit by bit, then the chunk
-__device__ __forceinline__ void find_bound(Shared& sh, int k) {
-  const int lane = threadIdx.x;
-  uint32_t key[WAVES];
-  int chunk[WAVES];
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    key[w] = sh.key[lane + 64 * w];
-    chunk[w] = sh.chunk[lane + 64 * w];
-  }
-  uint32_t bound = 0;
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t c = bound | (1u << b);
-    int n = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) n += __popcll(__ballot(key[w] >= c));
-    if (n >= k) bound = c;
-  }
-  int last = 0x7fffffff;
-  if (bound) {
-    int over = 0, equal = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      over += __popcll(__ballot(key[w] > bound));
-      equal += __popcll(__ballot(key[w] == bound));
-    }
-    if (over + equal > k) {  // the smallest `last` with k - over equal keys at or before it
-      last = 0;
-      for (int b = 30; b >= 0; --b) {
-        const int c = last + (1 << b);  // with fewer than k - over before c, the answer is c or later
-        int n = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) n += __popcll(__ballot(key[w] == bound && chunk[w] < c));
-        if (n < k - over) last = c;
-      }
-    }
-  }
-  if (lane == 0) {
-    sh.bound = bound;
-    sh.bound_chunk = last;
-  }
+__device__ __forceinline__ float max8(const float (&f)[8]) {
+  return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
 }
 
-// (m, s, t) of x[0, n), and its k best in sh.value / sh.index [0, k) in order, index -1 where there are no more; classes
-// are counted from `first`. Every thread returns the same Stat.
-template <int DT>
-__device__ Stat row_part(const typename mx_elem<DT>::type* __restrict__ x, int n, int first, int k, Shared& sh) {
-  const int tid = threadIdx.x, chunks = (n + 7) / 8;
-  Stat st = {LOWEST, 0.f, 0.f};
-  float best = -INFINITY;
-  int best_chunk = 0;
-  for (int c = tid; c < chunks; c += T) {
-    float f[8];
-    load_chunk<DT>(x, c * 8, n, f);
-    float cm = f[0];
+// s and t of 8 logits relative to st.m
+__device__ __forceinline__ void add8(Stat& st, const float (&f)[8]) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) cm = fmaxf(cm, f[i]);
-    best_chunk = cm > best ? c : best_chunk;
-    best = fmaxf(best, cm);
-    const float m = fmaxf(st.m, best), d = st.m - m, r = exp_(d);
-    st.t = r * (st.t + fmaxf(d, FAR) * st.s);
-    st.s *= r;
-    st.m = m;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float u = f[i] - m, e = exp_(u);
-      st.s += e;
-      st.t = fmaf(e, fmaxf(u, FAR), st.t);
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float u = f[i] - st.m, e = exp_(u);
+    st.s += e;
+    st.t = fmaf(e, fmaxf(u, FAR), st.t);
   }
-  const Stat w = wave_join(st);
-  if ((tid & 63) == 0) sh.stat[tid >> 6] = w;
-  sh.key[tid] = best > -INFINITY ? ordered(best) : 0;
-  sh.chunk[tid] = best_chunk;
-  if (tid == 0) sh.n_lanes = sh.n_cand = 0;
-  __syncthreads();
-  Stat all = sh.stat[0];
-#pragma unroll
-  for (int i = 1; i < WAVES; ++i) all = join(all, sh.stat[i]);
-  if (k == 0) return all;
-
-  if (tid < 64) find_bound(sh, k);
-  __syncthreads();
-  const uint32_t bound = sh.bound;
-  const int bound_chunk = sh.bound_chunk;
-  {
-    const uint32_t key = sh.key[tid];
-    if (key && (key > bound || (key == bound && best_chunk <= bound_chunk))) sh.lanes[atomicAdd(&sh.n_lanes, 1)] = tid;
-  }
-  __syncthreads();
-  const int per_lane = (chunks + T - 1) / T, items = sh.n_lanes * per_lane;
-  const float least = bound ? unordered(bound) : -INFINITY;
-  for (int it = tid; it < items; it += T) {
-    const int j = it / per_lane, c = sh.lanes[j] + (it - j * per_lane) * T;
-    if (c >= chunks) continue;
-    float f[8];
-    load_chunk<DT>(x, c * 8, n, f);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (f[i] > least || (f[i] == least && bound && c <= bound_chunk)) {
-        const int at = atomicAdd(&sh.n_cand, 1);
-        if (at < CAP) {
-          sh.value[at] = f[i];
-          sh.index[at] = first + c * 8 + i;
-        }
-      }
-  }
-  __syncthreads();
-  const int cand = sh.n_cand;
-  if (cand <= CAP) {
-    float v[CAP / T];
-    int id[CAP / T], rank[CAP / T];
-#pragma unroll
-    for (int q = 0; q < CAP / T; ++q) {
-      const int a = tid + q * T;
-      v[q] = a < cand ? sh.value[a] : 0.f;
-      id[q] = a < cand ? sh.index[a] : 0;
-      rank[q] = a < cand ? 0 : KMAX;
-    }
-    for (int b = 0; b < cand; ++b) {
-      const float bv = sh.value[b];
-      const int bi = sh.index[b];
-#pragma unroll
-      for (int q = 0; q < CAP / T; ++q) rank[q] += before(bv, bi, v[q], id[q]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < CAP / T; ++q)
-      if (rank[q] < k) {
-        sh.value[rank[q]] = v[q];
-        sh.index[rank[q]] = id[q];
-      }
-    if (tid >= cand && tid < k) {
-      sh.value[tid] = -INFINITY;
-      sh.index[tid] = -1;
-    }
-  } else {
-    float pv = INFINITY;  // the class that the last round found
-    int pi = -1;
-    for (int r = 0; r < k; ++r) {
-      float bv = -INFINITY;
-      int bi = 0x7fffffff;
-      for (int c = tid; c < chunks; c += T) {
-        float f[8];
-        load_chunk<DT>(x, c * 8, n, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int id = first + c * 8 + i;
-          if (f[i] > -INFINITY && before(pv, pi, f[i], id) && before(f[i], id, bv, bi)) {
-            bv = f[i];
-            bi = id;
-          }
-        }
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        const float ov = __shfl_xor(bv, o, 64);
-        const int oi = __shfl_xor(bi, o, 64);
-        if (before(ov, oi, bv, bi)) {
-          bv = ov;
-          bi = oi;
-        }
-      }
-      __syncthreads();  // the last round's (or the candidates') slots have been read
-      if ((tid & 63) == 0) {
-        sh.round_value[tid >> 6] = bv;
-        sh.round_index[tid >> 6] = bi;
-      }
-      __syncthreads();
-      pv = sh.round_value[0];
-      pi = sh.round_index[0];
-#pragma unroll
-      for (int w2 = 1; w2 < WAVES; ++w2)
-        if (before(sh.round_value[w2], sh.round_index[w2], pv, pi)) {
-          pv = sh.round_value[w2];
-          pi = sh.round_index[w2];
-        }
-      if (tid == 0) {
-        sh.value[r] = pv;
-        sh.index[r] = pi;
-      }
-    }
-  }
-  __syncthreads();
-  return all;
 }
 
 struct Out {
@@ -274,155 +111,352 @@ struct Out {
   float* top_logp;
 };
 
-// what a row answers. No finite logit: nothing is possible (log-probabilities -inf, entropy 0). A NaN or +inf among
-// them: no distribution (NaN, classes -1).
+// label j of a row: its logit, and whether it is below 0 (the row has none) or over the classes
+struct Label {
+  float x;
+  int kind;
+};
 template <int DT, typename L>
-__device__ __forceinline__ void answer(const Stat& st, const typename mx_elem<DT>::type* x, int c, const L* labels,
-                                       int n_labels, long row, int k, const float* value, const int* index,
-                                       const Out& out) {
-  const float log_s = logf(st.s);
-  const bool none = st.s == 0.f, bad = !(st.s < INFINITY);
-  const float nan = __uint_as_float(0x7fc00000u);
-  const int tid = threadIdx.x;
-  if (tid == 0) out.entropy[row] = none ? 0.f : bad ? nan : log_s - st.t / st.s;
-  for (int j = tid; j < n_labels; j += T) {
-    const long l = static_cast<long>(labels[row * n_labels + j]);
-    float v;
-    if (l < 0)
-      v = 0.f;  // no label
-    else if (l >= c || bad)
-      v = nan;
-    else
-      v = none ? -INFINITY : (mx_elem<DT>::one(x[l]) - st.m) - log_s;
-    out.logp[row * n_labels + j] = v;
+__device__ __forceinline__ Label label(const typename mx_elem<DT>::type* x, int c, const L* lab, int n, int j, long row) {
+  Label v = {0.f, -1};
+  if (j < n) {
+    const long l = static_cast<long>(lab[row * n + j]);
+    v.kind = l < 0 ? -1 : l >= c ? 1 : 0;
+    if (v.kind == 0) v.x = mx_elem<DT>::one(x[l]);
   }
-  for (int r = tid; r < k; r += T) {
-    out.top_idx[row * k + r] = bad ? -1 : index[r];
-    out.top_logp[row * k + r] = bad ? nan : index[r] < 0 ? -INFINITY : (value[r] - st.m) - log_s;
+  return v;
+}
+
+// What a row answers, from its sums. No finite logit: nothing is possible (log-probabilities -inf, entropy 0). A NaN or
+// +inf among them: no distribution (NaN, classes -1).
+struct Answer {
+  float m, log_s;
+  bool none, bad;
+  __device__ explicit Answer(const Stat& st) : m(st.m), log_s(logf(st.s)), none(st.s == 0.f), bad(!(st.s < INFINITY)) {}
+  static __device__ float nan() { return __uint_as_float(0x7fc00000u); }
+  __device__ float logp(float v) const { return bad ? nan() : none ? -INFINITY : (v - m) - log_s; }
+  // the entropy and the labels, by the lanes of one wave; `first` holds the first 64 labels' logits
+  template <int DT, typename L>
+  __device__ void labels(const Stat& st, const Label& first, const typename mx_elem<DT>::type* x, int c, const L* lab, int n,
+                         long row, const Out& out) const {
+    const int lane = threadIdx.x & 63;
+    if (lane == 0) out.entropy[row] = bad ? nan() : none ? 0.f : log_s - st.t / st.s;
+    Label v = first;
+    for (int j = lane; j < n; j += 64) {
+      if (j >= 64) v = label<DT, L>(x, c, lab, n, j, row);
+      out.logp[row * n + j] = v.kind < 0 ? 0.f : v.kind > 0 ? nan() : logp(v.x);
+    }
+  }
+  // alternative r: (v, class), class < 0 where there is none
+  __device__ void top(int r, float v, int id, long row, int k, const Out& out) const {
+    out.top_idx[row * k + r] = bad ? -1 : id;
+    out.top_logp[row * k + r] = id < 0 && !bad ? -INFINITY : logp(v);
+  }
+};
+
+template <int WAVES>
+struct Shared {
+  Stat stat[WAVES];
+  uint32_t key[GROUPS];  // each group's maximum (ordered; 0: it has seen nothing over -inf) and chunk
+  int chunk[GROUPS];
+  float least;           // the bound: a logit over it is a candidate, one equal to it up to chunk `last`
+  int last;
+  int groups[KMAX];      // the groups at or over the bound
+  int n_groups, n_cand;
+  uint64_t cand[CAP];    // candidates: the ordered logit, then the class counted down
+  float round_value[WAVES];
+  int round_index[WAVES];
+};
+
+// The bound that the k best groups (larger key, then the lower chunk, first) reach, and which they are, by one wave: the
+// key bit by bit, until exactly k groups reach it, then the chunk among equal keys.
+template <int WAVES>
+__device__ __forceinline__ void find_bound(Shared<WAVES>& sh, int k) {
+  constexpr int PER = GROUPS / 64;
+  const int lane = threadIdx.x & 63;
+  uint32_t key[PER];
+  int chunk[PER];
+#pragma unroll
+  for (int w = 0; w < PER; ++w) {
+    key[w] = sh.key[lane + 64 * w];
+    chunk[w] = sh.chunk[lane + 64 * w];
+  }
+  uint32_t bound = 0;
+  int reach = 0;
+  for (int b = 31; b >= 0 && reach != k; --b) {
+    const uint32_t c = bound | (1u << b);
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < PER; ++w) n += __popcll(__ballot(key[w] >= c));
+    if (n >= k) {
+      bound = c;
+      reach = n;
+    }
+  }
+  int last = 0x7fffffff;
+  if (bound && reach > k) {  // equal keys: the smallest `last` with enough of them at or before it
+    int over = 0;
+#pragma unroll
+    for (int w = 0; w < PER; ++w) over += __popcll(__ballot(key[w] > bound));
+    last = 0;
+    for (int b = 30; b >= 0; --b) {
+      const int c = last + (1 << b);  // with fewer than k - over before c, the answer is c or later
+      int n = 0;
+#pragma unroll
+      for (int w = 0; w < PER; ++w) n += __popcll(__ballot(key[w] == bound && chunk[w] < c));
+      if (n < k - over) last = c;
+    }
+  }
+  int at = 0;
+#pragma unroll
+  for (int w = 0; w < PER; ++w) {
+    const bool in = key[w] && (key[w] > bound || (key[w] == bound && chunk[w] <= last));
+    const unsigned long long mask = __ballot(in);
+    if (in) sh.groups[at + __popcll(mask & ((1ull << lane) - 1))] = lane + 64 * w;
+    at += __popcll(mask);
+  }
+  if (lane == 0) {
+    sh.least = bound ? unordered(bound) : -INFINITY;
+    sh.last = bound ? last : -1;
+    sh.n_groups = at;
+    sh.n_cand = 0;
   }
 }
 
-template <int DT, typename L>
-__global__ __launch_bounds__(T) void logprobs_kernel(const typename mx_elem<DT>::type* __restrict__ x, long ld, long rows,
-                                                     int c, const L* __restrict__ labels, int n_labels, int k, Out out) {
-  __shared__ Shared sh;
+// A workgroup of WAVES waves per row
+template <int DT, typename L, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_elem<DT>::type* __restrict__ x, long ld,
+                                                              long rows, int c, const L* __restrict__ labels,
+                                                              int n_labels, int k, Out out) {
+  constexpr int T = WAVES * 64, MEMBERS = T / GROUPS;
+  constexpr int U = 2;  // chunks in flight per lane; 4 take registers that waves need (4096 x 131072: 231 us, 2: 214)
+  __shared__ Shared<WAVES> sh;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int full = c / 8, chunks = (c + 7) / 8;
   for (long row = blockIdx.x; row < rows; row += gridDim.x) {
     const auto* xr = x + row * ld;
-    const Stat st = row_part<DT>(xr, c, 0, k, sh);
-    answer<DT, L>(st, xr, c, labels, n_labels, row, k, sh.value, sh.index, out);
+    Label first = {0.f, -1};
+    if (wave == 1) first = label<DT, L>(xr, c, labels, n_labels, lane, row);
+    Stat st = {LOWEST, 0.f, 0.f};
+    float best = -INFINITY;
+    int best_chunk = 0;
+    auto see = [&](const float (&f)[8], int at) {
+      const float cm = max8(f);
+      best_chunk = cm > best ? at : best_chunk;
+      best = fmaxf(best, cm);
+    };
+    for (int base = tid; base < full; base += U * T) {
+      mx_pack8<typename mx_elem<DT>::type> q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (base + u * T < full) q[u] = mx_load8<DT>(xr + (base + u * T) * 8l);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (base + u * T < full) {
+          float f[8];
+          mx_floats<DT>(q[u], f);
+          see(f, base + u * T);
+          st = rescaled(st, fmaxf(st.m, best));
+          add8(st, f);
+        }
+    }
+    if (chunks > full && tid == full % T) {
+      float f[8];
+      mx_load8_tail<DT>(xr + full * 8l, c - full * 8, -INFINITY, f);
+      see(f, full);
+      st = rescaled(st, fmaxf(st.m, best));
+      add8(st, f);
+    }
+    const Stat w = wave_join(st);
+    if (lane == 0) sh.stat[wave] = w;
+    if constexpr (MEMBERS == 4) {  // a group is four neighbouring lanes
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const float ob = s ? dpp<1>(best) : dpp<0>(best);
+        const int oc = s ? dpp<1>(best_chunk) : dpp<0>(best_chunk);
+        if (before(ob, oc, best, best_chunk)) {
+          best = ob;
+          best_chunk = oc;
+        }
+      }
+    }
+    if (tid % MEMBERS == 0) {
+      sh.key[tid / MEMBERS] = best > -INFINITY ? ordered(best) : 0;
+      sh.chunk[tid / MEMBERS] = best_chunk;
+    }
+    __syncthreads();
+    // the second wave finishes the labels while the first looks for the bound
+    if (wave == 0 && k > 0) find_bound(sh, k);
+    Stat all = {LOWEST, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) all.m = fmaxf(all.m, sh.stat[i].m);
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) {
+      const Stat r = rescaled(sh.stat[i], all.m);
+      all.s += r.s;
+      all.t += r.t;
+    }
+    const Answer ans(all);
+    if (wave == 1) ans.labels<DT, L>(all, first, xr, c, labels, n_labels, row, out);
+    if (k > 0) {
+      __syncthreads();
+      const float least = sh.least;
+      const int last = sh.last;
+      const int per = (chunks + T - 1) / T, items = sh.n_groups * MEMBERS * per;
+      for (int it = tid; it < items; it += T) {
+        const int lanes = it / per, at = sh.groups[lanes / MEMBERS] * MEMBERS + lanes % MEMBERS + (it - lanes * per) * T;
+        if (at >= chunks) continue;
+        float f[8];
+        load_chunk<DT>(xr, at * 8, c, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (f[i] > least || (f[i] == least && at <= last)) {
+            const int to = atomicAdd(&sh.n_cand, 1);
+            if (to < CAP) sh.cand[to] = static_cast<uint64_t>(ordered(f[i])) << 32 | ~static_cast<uint32_t>(at * 8 + i);
+          }
+      }
+      __syncthreads();
+      const int cand = sh.n_cand;
+      if (cand <= CAP) {
+        for (int a = tid; a < cand; a += T) {
+          const uint64_t key = sh.cand[a];
+          int rank = 0;
+          for (int b = 0; b < cand; ++b) rank += sh.cand[b] > key;
+          if (rank < k) ans.top(rank, unordered(key >> 32), ~static_cast<uint32_t>(key), row, k, out);
+        }
+        if (tid >= cand && tid < k) ans.top(tid, 0.f, -1, row, k, out);
+      } else {
+        float pv = INFINITY;  // the class that the last round found
+        int pi = -1;
+        for (int r = 0; r < k; ++r) {
+          float bv = -INFINITY;
+          int bi = 0x7fffffff;
+          for (int at = tid; at < chunks; at += T) {
+            float f[8];
+            load_chunk<DT>(xr, at * 8, c, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int id = at * 8 + i;
+              if (f[i] > -INFINITY && before(pv, pi, f[i], id) && before(f[i], id, bv, bi)) {
+                bv = f[i];
+                bi = id;
+              }
+            }
+          }
+          const float wv = wave_max(bv);
+          const int wi = wave_min(bv == wv ? bi : 0x7fffffff);
+          __syncthreads();  // the last round's slots have been read
+          if (lane == 0) {
+            sh.round_value[wave] = wv;
+            sh.round_index[wave] = wi;
+          }
+          __syncthreads();
+          pv = sh.round_value[0];
+          pi = sh.round_index[0];
+#pragma unroll
+          for (int i = 1; i < WAVES; ++i)
+            if (before(sh.round_value[i], sh.round_index[i], pv, pi)) {
+              pv = sh.round_value[i];
+              pi = sh.round_index[i];
+            }
+          if (tid == 0) ans.top(r, pv, pi, row, k, out);
+        }
+      }
+    }
     __syncthreads();  // the next row writes the shared parts
   }
 }
 
-// part p of a row: classes [p * len, (p + 1) * len); ws holds Stat [rows, splits], then k values and k classes of each
-template <int DT>
-__global__ __launch_bounds__(T) void logprobs_part_kernel(const typename mx_elem<DT>::type* __restrict__ x, long ld,
-                                                          int c, int splits, int len, int k, float* __restrict__ ws,
-                                                          float* __restrict__ wv, int* __restrict__ wi) {
-  __shared__ Shared sh;
-  const int row = blockIdx.x / splits, p = blockIdx.x - row * splits;
-  const int c0 = p * len, n = min(len, c - c0);
-  const Stat st = row_part<DT>(x + row * ld + c0, n, c0, k, sh);
-  if (threadIdx.x == 0) {
-    ws[blockIdx.x * 3] = st.m;
-    ws[blockIdx.x * 3 + 1] = st.s;
-    ws[blockIdx.x * 3 + 2] = st.t;
+// A wave per row of at most 512 CH classes, all in registers; an alternative is a wave's maximum, then retired
+template <int DT, typename L, int CH>
+__global__ __launch_bounds__(256) void logprobs_wave_kernel(const typename mx_elem<DT>::type* __restrict__ x, long ld,
+                                                            long rows, int c, const L* __restrict__ labels, int n_labels,
+                                                            int k, Out out) {
+  const int lane = threadIdx.x & 63;
+  const long row = static_cast<long>(blockIdx.x) * (blockDim.x >> 6) + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const auto* xr = x + row * ld;
+  const Label first = label<DT, L>(xr, c, labels, n_labels, lane, row);
+  float f[CH][8];
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    const int at = (j * 64 + lane) * 8;
+    if (at < c)
+      load_chunk<DT>(xr, at, c, f[j]);
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[j][i] = -INFINITY;
   }
-  if (static_cast<int>(threadIdx.x) < k) {
-    wv[blockIdx.x * k + threadIdx.x] = sh.value[threadIdx.x];
-    wi[blockIdx.x * k + threadIdx.x] = sh.index[threadIdx.x];
+  Stat st = {LOWEST, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < CH; ++j) st.m = fmaxf(st.m, max8(f[j]));
+  st.m = wave_max(st.m);
+#pragma unroll
+  for (int j = 0; j < CH; ++j) add8(st, f[j]);
+  st.s = wave_sum(st.s);
+  st.t = wave_sum(st.t);
+  const Answer ans(st);
+  ans.labels<DT, L>(st, first, xr, c, labels, n_labels, row, out);
+  for (int r = 0; r < k; ++r) {
+    float bv = -INFINITY;
+    int bi = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (f[j][i] > bv) {
+          bv = f[j][i];
+          bi = (j * 64 + lane) * 8 + i;
+        }
+    const float wv = wave_max(bv);
+    const int wi = wave_min(bv == wv ? bi : 0x7fffffff);
+    if (lane == 0) ans.top(r, wv, wv > -INFINITY ? wi : -1, row, k, out);
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if ((j * 64 + lane) * 8 + i == wi) f[j][i] = -INFINITY;
   }
 }
 
 template <int DT, typename L>
-__global__ __launch_bounds__(T) void logprobs_join_kernel(const typename mx_elem<DT>::type* __restrict__ x, long ld,
-                                                          int c, const L* __restrict__ labels, int n_labels, int splits,
-                                                          int k, const float* __restrict__ ws,
-                                                          const float* __restrict__ wv, const int* __restrict__ wi,
-                                                          Out out) {
-  __shared__ float value[SPLITS_MAX * KMAX];
-  __shared__ int index[SPLITS_MAX * KMAX];
-  __shared__ float top_value[KMAX];
-  __shared__ int top_index[KMAX];
-  const int row = blockIdx.x, tid = threadIdx.x, n = splits * k;
-  const float* w = ws + static_cast<long>(row) * splits * 3;
-  Stat st = {w[0], w[1], w[2]};
-  for (int p = 1; p < splits; ++p) st = join(st, {w[p * 3], w[p * 3 + 1], w[p * 3 + 2]});
-  for (int a = tid; a < n; a += T) {
-    value[a] = wv[static_cast<long>(row) * n + a];
-    index[a] = wi[static_cast<long>(row) * n + a];
-  }
-  if (tid < k) {
-    top_value[tid] = -INFINITY;
-    top_index[tid] = -1;
-  }
-  __syncthreads();
-  for (int a = tid; a < n; a += T) {
-    const float v = value[a];
-    const int id = index[a];
-    if (id < 0) continue;
-    int rank = 0;
-    for (int b = 0; b < n && rank < k; ++b) rank += index[b] >= 0 && before(value[b], index[b], v, id);
-    if (rank < k) {
-      top_value[rank] = v;
-      top_index[rank] = id;
-    }
-  }
-  __syncthreads();
-  answer<DT, L>(st, x + static_cast<long>(row) * ld, c, labels, n_labels, row, k, top_value, top_index, out);
-}
-
-// Parts per row: a row of fewer than 1024 is cut until 1024 workgroups are there or a part has 4096 classes.
-int splits_of(long rows, int c) {
-  const long want = (1024 + rows - 1) / rows, most = (c + 4095) / 4096;
-  const long n = want < most ? want : most;
-  return static_cast<int>(n < 1 ? 1 : n > SPLITS_MAX ? SPLITS_MAX : n);
-}
-
-template <int DT, typename L>
-void launch(const void* x, long ld, long rows, int c, const void* labels, int n_labels, int k, const Out& out, void* ws,
+void launch(const void* x, long ld, long rows, int c, const void* labels, int n_labels, int k, const Out& out,
             hipStream_t s) {
   const auto* xp = static_cast<const typename mx_elem<DT>::type*>(x);
   const auto* lp = static_cast<const L*>(labels);
-  const int splits = splits_of(rows, c);
-  if (splits == 1) {
-    hipLaunchKernelGGL((logprobs_kernel<DT, L>), dim3(static_cast<unsigned>(rows < (1 << 20) ? rows : (1 << 20))), dim3(T),
-                       0, s, xp, ld, rows, c, lp, n_labels, k, out);
+#define GO(KERNEL, GRID, BLOCK) hipLaunchKernelGGL((KERNEL), dim3(static_cast<unsigned>(GRID)), dim3(BLOCK), 0, s, xp, ld, rows, c, lp, n_labels, k, out)
+  if (c <= 2048 && k <= 16 && rows <= (1 << 24)) {
+    const int per = rows < 1024 ? 1 : 4;  // rows per workgroup
+    const long grid = (rows + per - 1) / per;
+    if (c <= 512) GO((logprobs_wave_kernel<DT, L, 1>), grid, per * 64);
+    else if (c <= 1024) GO((logprobs_wave_kernel<DT, L, 2>), grid, per * 64);
+    else GO((logprobs_wave_kernel<DT, L, 4>), grid, per * 64);
     return;
   }
-  const int parts = static_cast<int>(rows) * splits, len = ((c + splits - 1) / splits + 7) / 8 * 8;
-  float* st = static_cast<float*>(ws);
-  float* wv = st + parts * 3;
-  int* wi = reinterpret_cast<int*>(wv + parts * k);
-  hipLaunchKernelGGL((logprobs_part_kernel<DT>), dim3(parts), dim3(T), 0, s, xp, ld, c, splits, len, k, st, wv, wi);
-  hipLaunchKernelGGL((logprobs_join_kernel<DT, L>), dim3(static_cast<unsigned>(rows)), dim3(T), 0, s, xp, ld, c, lp, n_labels,
-                     splits, k, st, wv, wi, out);
+  const long grid = rows < (1 << 20) ? rows : (1 << 20);
+  // 16 waves see a row sooner (1 x 131072: 16.7 us against 22.9) where there are too few rows to fill the CUs with 4
+  // (1 x 32768: 11.3 against 9.4; 333 x 50001 fp32: 27 against 21)
+  if (rows <= 128 && c >= 65536) GO((logprobs_kernel<DT, L, 16>), grid, 1024);
+  else GO((logprobs_kernel<DT, L, 4>), grid, 256);
+#undef GO
 }
 
 }  // namespace
 
-// 4-byte words of workspace that ai4e_label_logprobs takes (0: none)
-AI4E_API int ai4e_label_logprobs_ws(long rows, int c, int k) {
-  if (rows <= 0 || c <= 0) return 0;
-  const int splits = splits_of(rows, c);
-  return splits == 1 ? 0 : static_cast<int>(rows) * splits * (3 + 2 * k);
-}
-
 // logits [rows, ld] of type dt (0 bf16, 1 fp16, 2 fp32), c valid columns; labels [rows, n_labels] int64 (wide) or int32;
 // logp [rows, n_labels], entropy [rows], top_idx / top_logp [rows, k], k <= 64 and <= c.
 AI4E_API int ai4e_label_logprobs(const void* logits, long ld, long rows, int c, int dt, const void* labels, int wide,
-                                 int n_labels, int k, void* logp, void* entropy, void* top_idx, void* top_logp, void* ws,
+                                 int n_labels, int k, void* logp, void* entropy, void* top_idx, void* top_logp,
                                  hipStream_t s) {
   if (!logits || !entropy || c <= 0 || c > (1 << 30) || ld < c || rows < 0 || dt < 0 || dt > 2 || k < 0 || k > KMAX || k > c ||
       n_labels < 0 || (n_labels && (!labels || !logp)) || (k && (!top_idx || !top_logp)))
     return AI4E_EINVAL;
   if (rows == 0) return AI4E_OK;
-  if (splits_of(rows, c) > 1 && !ws) return AI4E_EINVAL;
   const Out out = {static_cast<float*>(logp), static_cast<float*>(entropy), static_cast<int*>(top_idx),
                    static_cast<float*>(top_logp)};
-#define GO(DT)                                                                                       \
-  if (wide) launch<DT, int64_t>(logits, ld, rows, c, labels, n_labels, k, out, ws, s);               \
-  else launch<DT, int32_t>(logits, ld, rows, c, labels, n_labels, k, out, ws, s)
+#define GO(DT)                                                                                   \
+  if (wide) launch<DT, int64_t>(logits, ld, rows, c, labels, n_labels, k, out, s);               \
+  else launch<DT, int32_t>(logits, ld, rows, c, labels, n_labels, k, out, s)
   if (dt == MX_BF16) { GO(MX_BF16); }
   else if (dt == MX_F16) { GO(MX_F16); }
   else { GO(MX_F32); }

@@ -170,7 +170,5 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.ai4e_mx_linear(p, p, 0, p, None, None, 1, 1, 128, p, 0, None) == 1
     assert lib.ai4e_rms_norm_mx8(p, 4, None, 0, p, 0.0, 1, 4, 0, None, p, p, None) == 1
     assert lib.ai4e_rms_norm_mx8(p, 4, p, 3, p, 1e-6, 1, 4, 0, p, p, p, None) == 1
-    assert lib.ai4e_label_logprobs(p, 8, 1, 8, 0, p, 1, 1, 9, p, p, p, p, None, None) == 1   # k over the classes
-    assert lib.ai4e_label_logprobs(p, 8, 1, 8, 0, None, 1, 1, 0, p, p, None, None, None, None) == 1
-    assert lib.ai4e_label_logprobs(p, 1 << 20, 1, 1 << 20, 0, None, 0, 0, 0, None, p, None, None, None, None) == 1  # no workspace
-    assert lib.ai4e_label_logprobs_ws(0, 8, 1) == 0
+    assert lib.ai4e_label_logprobs(p, 8, 1, 8, 0, p, 1, 1, 9, p, p, p, p, None) == 1   # k over the classes
+    assert lib.ai4e_label_logprobs(p, 8, 1, 8, 0, None, 1, 1, 0, p, p, None, None, None) == 1
