@@ -321,7 +321,13 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
         for (int a = tid; a < cand; a += T) {
           const uint64_t key = sh.cand[a];
           int rank = 0;
-          for (int b = 0; b < cand; ++b) rank += sh.cand[b] > key;
+          for (int b = 0; b < cand; b += 8) {  // read together; what lies behind the last candidate does not count
+            uint64_t other[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) other[i] = sh.cand[b + i];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) rank += b + i < cand && other[i] > key;
+          }
           if (rank < k) ans.top(rank, unordered(key >> 32), ~static_cast<uint32_t>(key), row, k, out);
         }
         if (tid >= cand && tid < k) ans.top(tid, 0.f, -1, row, k, out);
@@ -434,9 +440,10 @@ void launch(const void* x, long ld, long rows, int c, const void* labels, int n_
     return;
   }
   const long grid = rows < (1 << 20) ? rows : (1 << 20);
-  // 16 waves see a row sooner (1 x 131072: 16.7 us against 22.9) where there are too few rows to fill the CUs with 4
-  // (1 x 32768: 11.3 against 9.4; 333 x 50001 fp32: 27 against 21)
-  if (rows <= 128 && c >= 65536) GO((logprobs_kernel<DT, L, 16>), grid, 1024);
+  // 16 waves per row where there are too few rows to fill the CUs with 4 (1 x 131072: 17.4 us against 22.8, 256 x 131072
+  // 24.8 against 40.4); with more rows their phases cost more (512 x 131072 45.7 against 45.3, 333 x 50001 fp32 25.8
+  // against 23.5, 1024 x 32768 47.6 against 25.2)
+  if (rows <= 256 && c >= 8192) GO((logprobs_kernel<DT, L, 16>), grid, 1024);
   else GO((logprobs_kernel<DT, L, 4>), grid, 256);
 #undef GO
 }
