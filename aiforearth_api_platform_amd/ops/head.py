@@ -51,26 +51,28 @@ def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, 
         raise ValueError("label_logprobs expects bfloat16, float16 or float32 logits of at least one class")
     if not 0 <= k <= min(c, MAX_ALTERNATIVES):
         raise ValueError(f"label_logprobs: k is 0 to {min(c, MAX_ALTERNATIVES)}, not {k}")
-    lead = logits.shape[:-1]
+    lead, index = logits.shape[:-1], logits.get_device()
+    n_labels = 0
     if labels is not None:
-        if labels.dtype not in (torch.int64, torch.int32) or labels.device != logits.device:
+        if labels.dtype not in (torch.int64, torch.int32) or labels.get_device() != index:
             raise ValueError("label_logprobs: labels are int64 or int32, on the logits' device")
-        if labels.shape != lead and labels.shape[:-1] != lead:
-            raise ValueError(f"label_logprobs: labels {tuple(labels.shape)} fit no logits {tuple(logits.shape)}")
+        shape = labels.shape
+        if shape != lead and (len(shape) == 0 or shape[:-1] != lead):
+            raise ValueError(f"label_logprobs: labels {tuple(shape)} fit no logits {tuple(logits.shape)}")
+        n_labels = 1 if shape == lead else shape[-1]
     _ext.refuse_grad("label_logprobs", logits)
-    n_labels = 0 if labels is None else 1 if labels.shape == lead else labels.shape[-1]
     if _ext.backend_for(logits) != "hip":
         return _label_logprobs_reference(logits, labels, n_labels, k)
     dev = logits.device
     logp = None if labels is None else torch.empty(labels.shape, device=dev, dtype=torch.float32)
     entropy = torch.empty(lead, device=dev, dtype=torch.float32)
-    top_idx = torch.empty(*lead, k, device=dev, dtype=torch.int32)
-    top_logp = torch.empty(*lead, k, device=dev, dtype=torch.float32)
+    top_idx = torch.empty((*lead, k), device=dev, dtype=torch.int32)
+    top_logp = torch.empty((*lead, k), device=dev, dtype=torch.float32)
     x = mx.rows_2d(logits)
     rows = x.shape[0]
     if rows:
         labels = None if labels is None else labels.contiguous()
-        _ext.call_on(dev, "ai4e_label_logprobs", x.data_ptr(), max(x.stride(0), c), rows, c, mx.DTYPE_CODE[x.dtype],
+        _ext.call_on(index, "ai4e_label_logprobs", x.data_ptr(), max(x.stride(0), c), rows, c, mx.DTYPE_CODE[x.dtype],
                      _ext.ptr(labels) if n_labels else None, int(n_labels > 0 and labels.dtype == torch.int64), n_labels, k,
                      _ext.ptr(logp), entropy.data_ptr(), top_idx.data_ptr(), top_logp.data_ptr())
     return LabelLogprobs(logp, entropy, top_idx, top_logp)

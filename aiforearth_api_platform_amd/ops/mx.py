@@ -56,29 +56,33 @@ def padded(k: int) -> int:
 def empty(lead, k: int, fmt: str, device) -> MxTensor:
     """An uninitialised MxTensor of ``(*lead, k)``."""
     kp = padded(k)
-    data = (torch.empty(*lead, kp, device=device, dtype=torch.float8_e4m3fn) if fmt == "e4m3"
-            else torch.empty(*lead, kp // 2, device=device, dtype=torch.uint8))
-    return MxTensor(data, torch.empty(*lead, kp // BLOCK, device=device, dtype=torch.float8_e8m0fnu), k)
+    data = (torch.empty((*lead, kp), device=device, dtype=torch.float8_e4m3fn) if fmt == "e4m3"
+            else torch.empty((*lead, kp // 2), device=device, dtype=torch.uint8))
+    return MxTensor(data, torch.empty((*lead, kp // BLOCK), device=device, dtype=torch.float8_e8m0fnu), k)
 
 
 def check(name: str, q: MxTensor) -> None:
     """Raises ValueError unless ``q`` has the layout that MxTensor describes."""
-    kp = padded(q.k)
-    if q.data.dtype not in (torch.uint8, torch.float8_e4m3fn) or q.scale.dtype not in (torch.uint8, torch.float8_e8m0fnu):
+    data, scale, k = q
+    e2m1 = data.dtype == torch.uint8
+    if not (e2m1 or data.dtype == torch.float8_e4m3fn) or scale.dtype not in (torch.uint8, torch.float8_e8m0fnu):
         raise ValueError(f"{name}: data is uint8 (e2m1) or float8_e4m3fn, scale float8_e8m0fnu or uint8")
-    if (q.k <= 0 or q.data.dim() < 1 or q.data.shape[:-1] != q.scale.shape[:-1] or q.scale.shape[-1] != kp // BLOCK
-            or q.data.shape[-1] != (kp // 2 if q.data.dtype == torch.uint8 else kp)):
-        raise ValueError(f"{name}: data {tuple(q.data.shape)} and scale {tuple(q.scale.shape)} do not hold rows of {q.k}")
-    if q.data.device != q.scale.device or not q.data.is_contiguous() or not q.scale.is_contiguous():
+    kp, shape, scales = padded(k), data.shape, scale.shape
+    if (k <= 0 or len(shape) < 1 or len(scales) < 1 or scales[-1] * BLOCK != kp or shape[-1] != (kp // 2 if e2m1 else kp)
+            or shape[:-1] != scales[:-1]):
+        raise ValueError(f"{name}: data {tuple(shape)} and scale {tuple(scales)} do not hold rows of {k}")
+    if data.get_device() != scale.get_device() or not data.is_contiguous() or not scale.is_contiguous():
         raise ValueError(f"{name}: data and scale have to be contiguous and on one device")
-    if q.data.data_ptr() % 16 or q.scale.data_ptr() % 4:
+    if data.data_ptr() % 16 or scale.data_ptr() % 4:
         raise ValueError(f"{name}: data has to be 16-byte aligned, scale 4-byte aligned")
 
 
 def rows_2d(t: torch.Tensor) -> torch.Tensor:
     """``[..., K]`` as ``[rows, K]`` with unit stride along K; a copy only where no view has that."""
-    t = t.reshape(-1, t.shape[-1]) if t.dim() != 2 else t
-    return t if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    pitch, step = t.stride()
+    return t if step == 1 and (pitch >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
 
 
 def quantize_reference(x: torch.Tensor, fmt: str) -> MxTensor:
@@ -127,7 +131,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "e2m1") -> MxTensor:
     k = x.shape[-1]
     q = empty(x.shape[:-1], k, fmt, x.device)
     x = rows_2d(x)
-    _ext.call_on(x.device, "ai4e_mx_quantize", x.data_ptr(), max(x.stride(0), k), x.shape[0], k, DTYPE_CODE[x.dtype],
+    _ext.call_on(x.get_device(), "ai4e_mx_quantize", x.data_ptr(), max(x.stride(0), k), x.shape[0], k, DTYPE_CODE[x.dtype],
                  FMT_CODE[fmt], q.data.data_ptr(), q.scale.data_ptr())
     return q
 
@@ -141,7 +145,7 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
         return dequantize_reference(q).to(dtype)
     y = torch.empty(q.shape, device=q.device, dtype=dtype)
     if y.numel():
-        _ext.call_on(q.device, "ai4e_mx_dequantize", q.data.data_ptr(), q.scale.data_ptr(), y.numel() // q.k, q.k,
+        _ext.call_on(y.get_device(), "ai4e_mx_dequantize", q.data.data_ptr(), q.scale.data_ptr(), y.numel() // q.k, q.k,
                      DTYPE_CODE[dtype], FMT_CODE[q.fmt], y.data_ptr())
     return y
 
@@ -156,27 +160,29 @@ def mx_linear(x: MxTensor, w: MxTensor, bias: Optional[torch.Tensor] = None,
     only."""
     check("mx_linear: x", x)
     check("mx_linear: w", w)
+    data, scale, k = x
+    fmt = x.fmt
     if w.fmt != "e2m1" or w.data.dim() != 2:
         raise ValueError("mx_linear: w is an e2m1 MxTensor [N, K]")
-    if x.k != w.k:
-        raise ValueError(f"mx_linear: x has rows of {x.k}, w of {w.k}")
+    if k != w.k:
+        raise ValueError(f"mx_linear: x has rows of {k}, w of {w.k}")
     if out_dtype not in DTYPE_CODE:
         raise ValueError("mx_linear gives bfloat16, float16 or float32")
-    if out_dtype == torch.float32 and x.fmt != "e2m1":
+    if out_dtype == torch.float32 and fmt != "e2m1":
         raise ValueError("mx_linear: float32 results need e2m1 activations (8-bit products are added to about 17 bits)")
     n = w.data.shape[0]
     if bias is not None and (tuple(bias.shape) != (n,) or not bias.is_floating_point()):
         raise ValueError(f"mx_linear: bias is a floating tensor of {n} values")
-    if w.device != x.device or (bias is not None and bias.device != x.device):
+    index = data.get_device()
+    if w.data.get_device() != index or (bias is not None and bias.get_device() != index):
         raise ValueError("mx_linear: x, w and bias have to be on one device")
     _ext.refuse_grad("mx_linear", bias)
-    lead = x.data.shape[:-1]
-    if _ext.backend_for(x.data) != "hip":
+    if _ext.backend_for(data) != "hip":
         y = dequantize_reference(x) @ dequantize_reference(w).T
         return (y if bias is None else y + bias.float()).to(out_dtype)
-    y = torch.empty(*lead, n, device=x.device, dtype=out_dtype)
+    y = torch.empty((*data.shape[:-1], n), device=data.device, dtype=out_dtype)
     if y.numel():
         b32 = None if bias is None else bias.to(torch.float32).contiguous()
-        _ext.call_on(x.device, "ai4e_mx_linear", x.data.data_ptr(), x.scale.data_ptr(), FMT_CODE[x.fmt], w.data.data_ptr(),
-                     w.scale.data_ptr(), _ext.ptr(b32), y.numel() // n, n, padded(x.k), y.data_ptr(), DTYPE_CODE[out_dtype])
+        _ext.call_on(index, "ai4e_mx_linear", data.data_ptr(), scale.data_ptr(), FMT_CODE[fmt], w.data.data_ptr(),
+                     w.scale.data_ptr(), _ext.ptr(b32), y.numel() // n, n, padded(k), y.data_ptr(), DTYPE_CODE[out_dtype])
     return y

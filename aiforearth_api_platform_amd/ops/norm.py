@@ -155,11 +155,12 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
     c = x.shape[-1] if x.dim() else 0
     if x.dtype not in mx.DTYPE_CODE or c == 0:
         raise ValueError("rms_norm_mx8 expects bfloat16, float16 or float32 with a last axis of at least one value")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+    shape, index = x.shape, x.get_device()
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("rms_norm_mx8: residual has to have x's shape and type")
-    if tuple(gamma.shape) != (c,) or not gamma.is_floating_point():
+    if gamma.dim() != 1 or gamma.shape[0] != c or not gamma.is_floating_point():
         raise ValueError(f"rms_norm_mx8: gamma is a floating tensor of {c} values")
-    if gamma.device != x.device or (residual is not None and residual.device != x.device):
+    if gamma.get_device() != index or (residual is not None and residual.get_device() != index):
         raise ValueError("rms_norm_mx8: x, gamma and residual have to be on one device")
     if not eps > 0:
         raise ValueError("rms_norm_mx8: eps has to be positive")
@@ -168,12 +169,12 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
         h = x.float() if residual is None else x.float() + residual.float()
         y = h.double() / torch.sqrt(h.double().square().mean(-1, keepdim=True) + eps) * gamma.double()
         return mx.quantize_reference(y.float(), "e4m3"), None if residual is None else h.to(x.dtype)
-    q = mx.empty(x.shape[:-1], c, "e4m3", x.device)
-    h = None if residual is None else torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    g32 = gamma.to(torch.float32).contiguous()
+    q = mx.empty(shape[:-1], c, "e4m3", x.device)
+    h = None if residual is None else torch.empty(shape, device=x.device, dtype=x.dtype)
+    g32 = gamma if gamma.dtype == torch.float32 and gamma.is_contiguous() else gamma.to(torch.float32).contiguous()
     x2 = mx.rows_2d(x)
     r2 = None if residual is None else mx.rows_2d(residual)
-    _ext.call_on(x.device, "ai4e_rms_norm_mx8", x2.data_ptr(), max(x2.stride(0), c), _ext.ptr(r2),
+    _ext.call_on(index, "ai4e_rms_norm_mx8", x2.data_ptr(), max(x2.stride(0), c), _ext.ptr(r2),
                  0 if r2 is None else max(r2.stride(0), c), g32.data_ptr(), eps, x2.shape[0], c, mx.DTYPE_CODE[x.dtype],
                  _ext.ptr(h), q.data.data_ptr(), q.scale.data_ptr())
     return q, h

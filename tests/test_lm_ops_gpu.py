@@ -68,7 +68,7 @@ def test_quantize_writes_its_rows_only():
     x = torch.randn(5, 200, generator=gen(2)).bfloat16().to(DEV)
     data = torch.full((5 * 256 + 512,), 0x5A, dtype=torch.uint8, device=DEV)
     scale = torch.full((5 * 8 + 64,), 0x5A, dtype=torch.uint8, device=DEV)
-    _ext.call_on(x.device, "ai4e_mx_quantize", x.data_ptr(), 200, 5, 200, 0, 0, data[256:].data_ptr(), scale[32:].data_ptr())
+    _ext.call_on(x.get_device(), "ai4e_mx_quantize", x.data_ptr(), 200, 5, 200, 0, 0, data[256:].data_ptr(), scale[32:].data_ptr())
     torch.cuda.synchronize()
     assert data[:256].eq(0x5A).all() and data[256 + 5 * 256:].eq(0x5A).all()
     assert scale[:32].eq(0x5A).all() and scale[32 + 40:].eq(0x5A).all()
@@ -143,7 +143,7 @@ def test_linear_writes_its_rows_only(m, n):
     g = gen(7)
     xq, wq = mx_quantize(torch.randn(m, 256, generator=g).to(DEV), "e4m3"), mx_quantize(torch.randn(n, 256, generator=g).to(DEV))
     buf = torch.full((m * n + 2048,), 7.0, dtype=torch.bfloat16, device=DEV)
-    _ext.call_on(buf.device, "ai4e_mx_linear", xq.data.data_ptr(), xq.scale.data_ptr(), 0, wq.data.data_ptr(),
+    _ext.call_on(buf.get_device(), "ai4e_mx_linear", xq.data.data_ptr(), xq.scale.data_ptr(), 0, wq.data.data_ptr(),
                  wq.scale.data_ptr(), None, m, n, 256, buf[1024:].data_ptr(), 0)
     torch.cuda.synchronize()
     assert buf[:1024].eq(7).all() and buf[1024 + m * n:].eq(7).all()
