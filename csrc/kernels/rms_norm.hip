@@ -2,30 +2,37 @@
 //
 //   h = x + residual            y = h / sqrt(mean(h^2) + eps) * gamma            (e4m3, scales) = mx(y), h kept
 //
-// One workgroup per row. The row stays in registers between the sum of squares and the products, so memory is what
-// bounds it: per value 2 + 2 B in, 2 B (h) and 1.03 B (codes, scales) out for 16-bit rows.
+// The row stays in registers between the sum of squares and the products, so memory is what bounds it: per value 2 + 2 B
+// in, 2 B (h) and 1.03 B (codes, scales) out for 16-bit rows. A workgroup per row, or for narrow rows the 16, 32 or 64
+// lanes that its chunks of 8 fill.
 // A value next to the border of two 8-bit neighbours falls to either side by the last bit of y, so y is computed to
 // one rounding: the row's factor as a double, split into a float and its remainder, and h * factor with its error.
 #include "mx.h"
 
 namespace {
 
-// sum over the workgroup's WAVES waves of a per-lane float (each lane's own sum has at most a row's share of squares),
-// added in double
-template <int WAVES>
+// sum over a row's LANES lanes of a per-lane float (a lane's own sum has at most a row's share of squares), in double
+template <int LANES>
 __device__ __forceinline__ double row_sum(float v, double* lds) {
   double s = v;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-  if constexpr (WAVES > 1) {
+  for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if constexpr (LANES > 64) {
     __syncthreads();  // the last row's sums have been read
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
     __syncthreads();
     s = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) s += lds[w];
+    for (int w = 0; w < LANES / 64; ++w) s += lds[w];
   }
   return s;
+}
+
+// 1 / sqrt(d): the float estimate and a Newton step in double (to 2^-44) where the estimate is in range
+__device__ __forceinline__ double inv_sqrt(double d) {
+  if (!(d > 1e-30 && d < 1e38)) return 1.0 / sqrt(d);
+  const double r = __builtin_amdgcn_rsqf(static_cast<float>(d));
+  return r * (1.5 - 0.5 * d * r * r);
 }
 
 template <int DT>
@@ -50,40 +57,41 @@ __device__ __forceinline__ void load_h(const typename mx_elem<DT>::type* x, cons
   }
 }
 
-// CH > 0: the row's chunks of 8 per lane, kept in registers; CH == 0: any width, read a second time
-template <int DT, int WAVES, int CH>
-__global__ __launch_bounds__(WAVES * 64) void rms_norm_mx8_kernel(
+// LANES lanes per row; CH > 0: the row's chunks of 8 per lane, kept in registers; CH == 0: any width, read a second time
+template <int DT, int LANES, int CH>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_mx8_kernel(
     const typename mx_elem<DT>::type* __restrict__ x, long ldx, const typename mx_elem<DT>::type* __restrict__ res,
-    long ldr, const float* __restrict__ gamma, float eps, long rows, int c, int cp,
+    long ldr, const float* __restrict__ gamma, float eps, double inv_c, long rows, int c, int cp,
     typename mx_elem<DT>::type* __restrict__ hout, uint8_t* __restrict__ data, uint8_t* __restrict__ scale) {
-  constexpr int T = WAVES * 64;
+  constexpr int T = LANES > 256 ? LANES : 256, ROWS = T / LANES;
+  static_assert(LANES <= 64 || ROWS == 1, "rows of several waves share no workgroup: they meet at its barriers");
   constexpr int KEEP = CH > 0 ? CH : 1;
-  __shared__ double lds[WAVES];
-  const int tid = threadIdx.x;
-  const int nch = CH > 0 ? CH : (cp / 8 + T - 1) / T;
-  for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+  __shared__ double lds[T / 64];
+  const int tid = threadIdx.x % LANES;
+  const int nch = CH > 0 ? CH : (cp / 8 + LANES - 1) / LANES;
+  for (long row = static_cast<long>(blockIdx.x) * ROWS + threadIdx.x / LANES; row < rows; row += static_cast<long>(gridDim.x) * ROWS) {
     const auto* xr = x + row * ldx;
     const auto* rr = res ? res + row * ldr : nullptr;
     float h[KEEP][8];
     float sq = 0.f;
 #pragma unroll
     for (int j = 0; j < nch; ++j) {
-      const int col = (j * T + tid) * 8;
+      const int col = (j * LANES + tid) * 8;
       float(&v)[8] = h[CH > 0 ? j : 0];
       load_h<DT>(xr + col, rr ? rr + col : nullptr, c - col, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
       if (hout && col < c) mx_store8<DT>(hout + row * c + col, v, c - col);
     }
-    double ms = row_sum<WAVES>(sq, lds);
+    double ms = row_sum<LANES>(sq, lds);
     double factor;
     if (ms < 3e38) {
-      factor = 1.0 / sqrt(ms / c + static_cast<double>(eps));
+      factor = inv_sqrt(ms * inv_c + static_cast<double>(eps));
     } else {  // the squares left 32 bits (or are not finite): once more, scaled by 2^-80
       sq = 0.f;
 #pragma unroll
       for (int j = 0; j < nch; ++j) {
-        const int col = (j * T + tid) * 8;
+        const int col = (j * LANES + tid) * 8;
         float(&v)[8] = h[CH > 0 ? j : 0];
         if (CH == 0) load_h<DT>(xr + col, rr ? rr + col : nullptr, c - col, v);
 #pragma unroll
@@ -92,13 +100,13 @@ __global__ __launch_bounds__(WAVES * 64) void rms_norm_mx8_kernel(
           sq = fmaf(u, u, sq);
         }
       }
-      ms = row_sum<WAVES>(sq, lds);
-      factor = 1.0 / (sqrt(ms / c + static_cast<double>(eps) * 0x1p-160) * 0x1p80);
+      ms = row_sum<LANES>(sq, lds);
+      factor = 1.0 / (sqrt(ms * inv_c + static_cast<double>(eps) * 0x1p-160) * 0x1p80);
     }
     const float fh = static_cast<float>(factor), fl = static_cast<float>(factor - static_cast<double>(fh));
 #pragma unroll
     for (int j = 0; j < nch; ++j) {
-      const int col = (j * T + tid) * 8;
+      const int col = (j * LANES + tid) * 8;
       if (col >= cp) break;  // cp is a multiple of 128: a block's four lanes leave together
       float(&v)[8] = h[CH > 0 ? j : 0];
       if (CH == 0) load_h<DT>(xr + col, rr ? rr + col : nullptr, c - col, v);
@@ -114,7 +122,7 @@ __global__ __launch_bounds__(WAVES * 64) void rms_norm_mx8_kernel(
       }
       const int code = mx_scale_code<MX_E4M3>(mx_quad_max(mx_abs_bits8(y)));
       const long at = row * cp + col;
-      *reinterpret_cast<uint2*>(data + at) = mx_pack_e4m3(y, code);
+      mx_store_past(reinterpret_cast<uint2*>(data + at), mx_pack_e4m3(y, code));
       if ((tid & 3) == 0) scale[at >> 5] = static_cast<uint8_t>(code);
     }
   }
@@ -131,17 +139,27 @@ AI4E_API int ai4e_rms_norm_mx8(const void* x, long ldx, const void* residual, lo
     return AI4E_EINVAL;
   if (rows == 0) return AI4E_OK;
   const int cp = ai4e_cdiv(c, MX_ALIGN) * MX_ALIGN;
-  const dim3 grid(static_cast<unsigned>(rows < (1 << 20) ? rows : (1 << 20)));
-#define GO(DT, W, CH)                                                                                            \
-  hipLaunchKernelGGL((rms_norm_mx8_kernel<DT, W, CH>), grid, dim3(W * 64), 0, s,                                 \
-                     static_cast<const mx_elem<DT>::type*>(x), ldx, static_cast<const mx_elem<DT>::type*>(residual), \
-                     ldr, static_cast<const float*>(gamma), eps, rows, c, cp, static_cast<mx_elem<DT>::type*>(hout), \
-                     static_cast<uint8_t*>(data), static_cast<uint8_t*>(scale))
-#define PICK(DT)                  \
-  if (cp <= 512) GO(DT, 1, 1);    \
-  else if (cp <= 2048) GO(DT, 4, 1); \
-  else if (cp <= 8192) GO(DT, 8, 2); \
-  else GO(DT, 8, 0)
+#define GO(DT, LANES, CH)                                                                                        \
+  {                                                                                                              \
+    constexpr int T = LANES > 256 ? LANES : 256;                                                                 \
+    const long blocks = (rows + T / LANES - 1) / (T / LANES);                                                    \
+    hipLaunchKernelGGL((rms_norm_mx8_kernel<DT, LANES, CH>), dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : (1 << 20))), \
+                       dim3(T), 0, s, static_cast<const mx_elem<DT>::type*>(x), ldx,                             \
+                       static_cast<const mx_elem<DT>::type*>(residual), ldr, static_cast<const float*>(gamma), eps, 1.0 / c, \
+                       rows, c, cp, static_cast<mx_elem<DT>::type*>(hout), static_cast<uint8_t*>(data),          \
+                       static_cast<uint8_t*>(scale));                                                            \
+  }
+// up to 8192 values a row takes as few lanes as hold it in two chunks each: 16384 x 8192 bf16 with 256 lanes x 4 chunks
+// 184 us, 512 x 2 173, 1024 x 1 243; 4096 x 4096 256 x 2 21.8, 512 x 1 22.9
+#define PICK(DT)                       \
+  if (cp <= 128) GO(DT, 16, 1)         \
+  else if (cp <= 256) GO(DT, 32, 1)    \
+  else if (cp <= 512) GO(DT, 64, 1)    \
+  else if (cp <= 2048) GO(DT, 256, 1)  \
+  else if (cp <= 4096) GO(DT, 256, 2)  \
+  else if (cp <= 8192) GO(DT, 512, 2)  \
+  else if (cp <= 16384) GO(DT, 512, 4) \
+  else GO(DT, 512, 0)
   if (dt == MX_BF16) { PICK(MX_BF16); }
   else if (dt == MX_F16) { PICK(MX_F16); }
   else { PICK(MX_F32); }

@@ -202,7 +202,7 @@ def check_norm(x, gamma, residual, eps=1e-6):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("c", [1, 8, 31, 32, 33, 128, 500, 512, 513, 2048, 2050, 4096, 5000, 8192, 8193, 20000])
+@pytest.mark.parametrize("c", [1, 8, 31, 32, 33, 128, 200, 500, 512, 513, 2048, 2050, 4096, 5000, 8192, 8193, 20000])
 def test_rms_norm(dtype, c):
     g = gen(c)
     for rows, with_residual in ((1, True), (3, False), (37, True)):
