@@ -82,7 +82,7 @@ __global__ __launch_bounds__(THREADS) void dequantize_kernel(const uint8_t* __re
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int c = at[i].col8 * 8;
-    if (at[i].row >= rows || c >= k) continue;
+    if (at[i].row >= rows) continue;
     const float s = scale_value(code[i]);
     float f[8];
     if constexpr (FMT == MX_E4M3) {
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(THREADS) void dequantize_kernel(const uint8_t* __re
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] *= s;
-    mx_store8<DT>(y + at[i].row * k + c, f, k - c);
+    mx_store8_quad<DT>(y + at[i].row * k, c, k, f);
   }
 }
 

@@ -81,7 +81,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_mx8_kernel
       load_h<DT>(xr + col, rr ? rr + col : nullptr, c - col, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
-      if (hout && col < c) mx_store8<DT>(hout + row * c + col, v, c - col);
+      if (hout) mx_store8_quad<DT>(hout + row * c, col, c, v);
     }
     double ms = row_sum<LANES>(sq, lds);
     double factor;
