@@ -4,9 +4,10 @@
 //   m = max x_j     s = sum e^(x_j - m)     t = sum e^(x_j - m) (x_j - m)
 //   logp(j) = x_j - m - log s               entropy = log s - t / s
 //
-// One pass: a lane keeps (m, s, t) of the elements it has seen and rescales s and t when its maximum grows, so a logit
-// is read once and memory bounds the kernel on large inputs, the row's phases on small ones. The differences x - m are
-// taken before the change to base 2: masks of the type's lowest value stay finite, and -inf gives e = 0.
+// One pass: a lane keeps its maximum, s and t of the elements it has seen and rescales s and t when the maximum grows, so
+// a logit is read once. The pass works in base 2, s = sum 2^d and t = sum 2^d d with d = x log2 e - mu in one fused
+// operation, mu the rounded m log2 e: what mu lost is put back at the end. -inf gives 2^d = 0. Where m log2 e leaves 32
+// bits (every logit is the type's lowest value, say) s ends as 0 and the row is summed again from differences x - m.
 //
 // The k best come out of the same pass (logprobs_kernel). A lane also keeps its best chunk (8 consecutive logits; the
 // first one with the lane's maximum). The k-th largest of 256 groups' (maximum, chunk) pairs bounds the k-th best logit
@@ -14,24 +15,27 @@
 // the bound is put into LDS, and each candidate's rank is the number of candidates before it. Ties go to the lower class.
 // If more candidates come than LDS has room for (their order on the row is adverse), k rounds over the row find one each.
 // Short rows with few alternatives stay in one wave's registers (logprobs_wave_kernel).
+#include <type_traits>
+
 #include "mx.h"
 
 namespace {
 
 constexpr int KMAX = 64, CAP = 1024, GROUPS = 256;
-constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LOWEST = -3.402823466e38f;
-constexpr float FAR = -200.f;  // e^FAR is 0 in 32 bits; keeps 0 * (x - m) from being 0 * -inf
+constexpr float FAR = -200.f;  // 2^FAR is 0 in 32 bits; keeps 0 * d from being 0 * -inf
 
+// the largest logit (-inf: none yet) and the sums relative to it
 struct Stat {
   float m, s, t;
 };
 
-__device__ __forceinline__ float exp_(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
+__device__ __forceinline__ float mu_of(float m) { return fmaxf(m * LOG2E, LOWEST); }
 
-// v's sums relative to a maximum m >= v.m
+// v's sums (base 2) relative to a maximum m >= v.m
 __device__ __forceinline__ Stat rescaled(const Stat& v, float m) {
-  const float d = v.m - m, f = exp_(d);
+  const float d = mu_of(v.m) - mu_of(m), f = __builtin_amdgcn_exp2f(d);
   return {m, v.s * f, f * (v.t + fmaxf(d, FAR) * v.s)};
 }
 
@@ -90,15 +94,31 @@ __device__ __forceinline__ void load_chunk(const typename mx_elem<DT>::type* x, 
     mx_load8_tail<DT>(x + c, n - c, -INFINITY, f);
 }
 
+// v_max3_f32 as such: from raw bits the compiler would quiet every operand first, an instruction each
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 __device__ __forceinline__ float max8(const float (&f)[8]) {
-  return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+  const float a = max3(f[0], f[1], f[2]), b = max3(f[3], f[4], f[5]);
+  return max3(max3(a, f[6], f[7]), b, b);
 }
 
-// s and t of 8 logits relative to st.m
-__device__ __forceinline__ void add8(Stat& st, const float (&f)[8]) {
+// s and t of 8 logits, base 2, relative to mu
+__device__ __forceinline__ void add8(Stat& st, const float (&f)[8], float mu) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float u = f[i] - st.m, e = exp_(u);
+    const float d = fmaf(f[i], LOG2E, -mu), e = __builtin_amdgcn_exp2f(d);
+    st.s += e;
+    st.t = fmaf(e, fmaxf(d, FAR), st.t);
+  }
+}
+// the same from differences, base e: for any finite maximum
+__device__ __forceinline__ void add8_differences(Stat& st, const float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float u = f[i] - st.m, e = __builtin_amdgcn_exp2f(u * LOG2E);
     st.s += e;
     st.t = fmaf(e, fmaxf(u, FAR), st.t);
   }
@@ -116,11 +136,18 @@ struct Label {
   float x;
   int kind;
 };
-template <int DT, typename L>
-__device__ __forceinline__ Label label(const typename mx_elem<DT>::type* x, int c, const L* lab, int n, int j, long row) {
+// the labels of all rows, n of each, int64 or int32
+struct Labels {
+  const void* p;
+  int n;
+  bool wide;
+};
+template <int DT>
+__device__ __forceinline__ Label label(const typename mx_elem<DT>::type* x, int c, const Labels& lab, int j, long row) {
   Label v = {0.f, -1};
-  if (j < n) {
-    const long l = static_cast<long>(lab[row * n + j]);
+  if (j < lab.n) {
+    const long at = row * lab.n + j;
+    const long l = lab.wide ? static_cast<const int64_t*>(lab.p)[at] : static_cast<const int32_t*>(lab.p)[at];
     v.kind = l < 0 ? -1 : l >= c ? 1 : 0;
     if (v.kind == 0) v.x = mx_elem<DT>::one(x[l]);
   }
@@ -130,21 +157,26 @@ __device__ __forceinline__ Label label(const typename mx_elem<DT>::type* x, int 
 // What a row answers, from its sums. No finite logit: nothing is possible (log-probabilities -inf, entropy 0). A NaN or
 // +inf among them: no distribution (NaN, classes -1).
 struct Answer {
-  float m, log_s;
+  float m, log_s, entropy;
   bool none, bad;
-  __device__ explicit Answer(const Stat& st) : m(st.m), log_s(logf(st.s)), none(st.s == 0.f), bad(!(st.s < INFINITY)) {}
+  __device__ Answer(const Stat& st, bool differences)
+      : m(st.m), none(st.m == -INFINITY), bad(!(st.s < INFINITY)) {
+    const float ln = logf(st.s);
+    log_s = differences ? ln : ln - fmaf(m, LOG2E, -mu_of(m)) * LN2;
+    entropy = differences ? ln - st.t / st.s : ln - st.t / st.s * LN2;
+  }
   static __device__ float nan() { return __uint_as_float(0x7fc00000u); }
   __device__ float logp(float v) const { return bad ? nan() : none ? -INFINITY : (v - m) - log_s; }
   // the entropy and the labels, by the lanes of one wave; `first` holds the first 64 labels' logits
-  template <int DT, typename L>
-  __device__ void labels(const Stat& st, const Label& first, const typename mx_elem<DT>::type* x, int c, const L* lab, int n,
-                         long row, const Out& out) const {
+  template <int DT>
+  __device__ void labels(const Label& first, const typename mx_elem<DT>::type* x, int c, const Labels& lab, long row,
+                         const Out& out) const {
     const int lane = threadIdx.x & 63;
-    if (lane == 0) out.entropy[row] = bad ? nan() : none ? 0.f : log_s - st.t / st.s;
+    if (lane == 0) out.entropy[row] = bad ? nan() : none ? 0.f : entropy;
     Label v = first;
-    for (int j = lane; j < n; j += 64) {
-      if (j >= 64) v = label<DT, L>(x, c, lab, n, j, row);
-      out.logp[row * n + j] = v.kind < 0 ? 0.f : v.kind > 0 ? nan() : logp(v.x);
+    for (int j = lane; j < lab.n; j += 64) {
+      if (j >= 64) v = label<DT>(x, c, lab, j, row);
+      out.logp[row * lab.n + j] = v.kind < 0 ? 0.f : v.kind > 0 ? nan() : logp(v.x);
     }
   }
   // alternative r: (v, class), class < 0 where there is none
@@ -223,50 +255,68 @@ __device__ __forceinline__ void find_bound(Shared<WAVES>& sh, int k) {
   }
 }
 
-// A workgroup of WAVES waves per row
-template <int DT, typename L, int WAVES>
+// A workgroup of WAVES waves per row. Its loads go through the caches, though 1 GB reads faster past them (7.1 TB/s, 6.3):
+// candidates are read again, and logits are often what the last kernel wrote (333 x 50001 fp32 18.5 us, past the caches
+// 28; 4096 x 131072 bf16 216 and 205).
+template <int DT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_elem<DT>::type* __restrict__ x, long ld,
-                                                              long rows, int c, const L* __restrict__ labels,
-                                                              int n_labels, int k, Out out) {
+                                                              long rows, int c, Labels labels, int k, Out out) {
   constexpr int T = WAVES * 64, MEMBERS = T / GROUPS;
-  constexpr int U = 2;  // chunks in flight per lane; 4 take registers that waves need (4096 x 131072: 231 us, 2: 214)
+  constexpr int U = 2;  // chunks per step and lane, the next step's in flight
   __shared__ Shared<WAVES> sh;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int full = c / 8, chunks = (c + 7) / 8;
   for (long row = blockIdx.x; row < rows; row += gridDim.x) {
     const auto* xr = x + row * ld;
     Label first = {0.f, -1};
-    if (wave == 1) first = label<DT, L>(xr, c, labels, n_labels, lane, row);
-    Stat st = {LOWEST, 0.f, 0.f};
-    float best = -INFINITY;
+    if (wave == 1) first = label<DT>(xr, c, labels, lane, row);
+    Stat st = {-INFINITY, 0.f, 0.f};
     int best_chunk = 0;
-    auto see = [&](const float (&f)[8], int at) {
-      const float cm = max8(f);
-      best_chunk = cm > best ? at : best_chunk;
-      best = fmaxf(best, cm);
+    typedef mx_raw8<DT> Pack;
+    // N chunks' logits, one rescaling for all
+    auto take = [&](auto count, const Pack* q, int at) {
+      constexpr int N = decltype(count)::value;
+      float f[N][8], m = st.m;
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        mx_floats<DT>(q[u], f[u]);
+        const float cm = max8(f[u]);
+        best_chunk = cm > m ? at + u * T : best_chunk;
+        m = fmaxf(m, cm);
+      }
+      st = rescaled(st, m);
+#pragma unroll
+      for (int u = 0; u < N; ++u) add8(st, f[u], mu_of(m));
     };
-    for (int base = tid; base < full; base += U * T) {
-      mx_pack8<typename mx_elem<DT>::type> q[U];
+    const int steps = full / (U * T);
+    if (steps > 0) {
+      Pack q[U];
+      auto fetch = [&](Pack(&p)[U], int step) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (base + u * T < full) q[u] = mx_load8<DT>(xr + (base + u * T) * 8l);
+        for (int u = 0; u < U; ++u) p[u] = mx_load8<DT>(xr + ((step * U + u) * T + tid) * 8l);
+      };
+      fetch(q, 0);
+      for (int i = 0; i < steps; ++i) {
+        Pack next[U];
+        if (i + 1 < steps) fetch(next, i + 1);
+        take(std::integral_constant<int, U>{}, q, i * U * T + tid);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (base + u * T < full) {
-          float f[8];
-          mx_floats<DT>(q[u], f);
-          see(f, base + u * T);
-          st = rescaled(st, fmaxf(st.m, best));
-          add8(st, f);
-        }
+        for (int u = 0; u < U; ++u) q[u] = next[u];
+      }
+    }
+    for (int at = steps * U * T + tid; at < full; at += T) {
+      const Pack q = mx_load8<DT>(xr + at * 8l);
+      take(std::integral_constant<int, 1>{}, &q, at);
     }
     if (chunks > full && tid == full % T) {
       float f[8];
       mx_load8_tail<DT>(xr + full * 8l, c - full * 8, -INFINITY, f);
-      see(f, full);
-      st = rescaled(st, fmaxf(st.m, best));
-      add8(st, f);
+      const float cm = max8(f);
+      best_chunk = cm > st.m ? full : best_chunk;
+      st = rescaled(st, fmaxf(st.m, cm));
+      add8(st, f, mu_of(st.m));
     }
+    float best = st.m;
     const Stat w = wave_join(st);
     if (lane == 0) sh.stat[wave] = w;
     if constexpr (MEMBERS == 4) {  // a group is four neighbouring lanes
@@ -287,7 +337,7 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
     __syncthreads();
     // the second wave finishes the labels while the first looks for the bound
     if (wave == 0 && k > 0) find_bound(sh, k);
-    Stat all = {LOWEST, 0.f, 0.f};
+    Stat all = {-INFINITY, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) all.m = fmaxf(all.m, sh.stat[i].m);
 #pragma unroll
@@ -296,8 +346,28 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
       all.s += r.s;
       all.t += r.t;
     }
-    const Answer ans(all);
-    if (wave == 1) ans.labels<DT, L>(all, first, xr, c, labels, n_labels, row, out);
+    const bool again = all.s == 0.f && all.m > -INFINITY;
+    if (again) {  // m log2 e is out of range
+      Stat d = {all.m, 0.f, 0.f};
+      for (int at = tid; at < chunks; at += T) {
+        float f[8];
+        load_chunk<DT>(xr, at * 8, c, f);
+        add8_differences(d, f);
+      }
+      d.s = wave_sum(d.s);
+      d.t = wave_sum(d.t);
+      __syncthreads();  // every wave has read the first sums
+      if (lane == 0) sh.stat[wave] = d;
+      __syncthreads();
+      all.t = 0.f;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) {
+        all.s += sh.stat[i].s;
+        all.t += sh.stat[i].t;
+      }
+    }
+    const Answer ans(all, again);
+    if (wave == 1) ans.labels<DT>(first, xr, c, labels, row, out);
     if (k > 0) {
       __syncthreads();
       const float least = sh.least;
@@ -374,15 +444,14 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
 }
 
 // A wave per row of at most 512 CH classes, all in registers; an alternative is a wave's maximum, then retired
-template <int DT, typename L, int CH>
+template <int DT, int CH>
 __global__ __launch_bounds__(256) void logprobs_wave_kernel(const typename mx_elem<DT>::type* __restrict__ x, long ld,
-                                                            long rows, int c, const L* __restrict__ labels, int n_labels,
-                                                            int k, Out out) {
+                                                            long rows, int c, Labels labels, int k, Out out) {
   const int lane = threadIdx.x & 63;
   const long row = static_cast<long>(blockIdx.x) * (blockDim.x >> 6) + (threadIdx.x >> 6);
   if (row >= rows) return;
   const auto* xr = x + row * ld;
-  const Label first = label<DT, L>(xr, c, labels, n_labels, lane, row);
+  const Label first = label<DT>(xr, c, labels, lane, row);
   float f[CH][8];
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
@@ -393,16 +462,23 @@ __global__ __launch_bounds__(256) void logprobs_wave_kernel(const typename mx_el
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[j][i] = -INFINITY;
   }
-  Stat st = {LOWEST, 0.f, 0.f};
+  Stat st = {-INFINITY, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < CH; ++j) st.m = fmaxf(st.m, max8(f[j]));
   st.m = wave_max(st.m);
+  if (st.m == -INFINITY) {  // nothing but -inf and NaN: a difference would be NaN for either
 #pragma unroll
-  for (int j = 0; j < CH; ++j) add8(st, f[j]);
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) st.s += f[j][i] == -INFINITY ? 0.f : f[j][i];
+  } else {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) add8_differences(st, f[j]);
+  }
   st.s = wave_sum(st.s);
   st.t = wave_sum(st.t);
-  const Answer ans(st);
-  ans.labels<DT, L>(st, first, xr, c, labels, n_labels, row, out);
+  const Answer ans(st, true);
+  ans.labels<DT>(first, xr, c, labels, row, out);
   for (int r = 0; r < k; ++r) {
     float bv = -INFINITY;
     int bi = 0x7fffffff;
@@ -425,26 +501,25 @@ __global__ __launch_bounds__(256) void logprobs_wave_kernel(const typename mx_el
   }
 }
 
-template <int DT, typename L>
-void launch(const void* x, long ld, long rows, int c, const void* labels, int n_labels, int k, const Out& out,
-            hipStream_t s) {
+template <int DT>
+void launch(const void* x, long ld, long rows, int c, const Labels& labels, int k, const Out& out, hipStream_t s) {
   const auto* xp = static_cast<const typename mx_elem<DT>::type*>(x);
-  const auto* lp = static_cast<const L*>(labels);
-#define GO(KERNEL, GRID, BLOCK) hipLaunchKernelGGL((KERNEL), dim3(static_cast<unsigned>(GRID)), dim3(BLOCK), 0, s, xp, ld, rows, c, lp, n_labels, k, out)
+#define GO(GRID, BLOCK, ...) \
+  hipLaunchKernelGGL((__VA_ARGS__), dim3(static_cast<unsigned>(GRID)), dim3(BLOCK), 0, s, xp, ld, rows, c, labels, k, out)
   if (c <= 2048 && k <= 16 && rows <= (1 << 24)) {
     const int per = rows < 1024 ? 1 : 4;  // rows per workgroup
     const long grid = (rows + per - 1) / per;
-    if (c <= 512) GO((logprobs_wave_kernel<DT, L, 1>), grid, per * 64);
-    else if (c <= 1024) GO((logprobs_wave_kernel<DT, L, 2>), grid, per * 64);
-    else GO((logprobs_wave_kernel<DT, L, 4>), grid, per * 64);
+    if (c <= 512) GO(grid, per * 64, logprobs_wave_kernel<DT, 1>);
+    else if (c <= 1024) GO(grid, per * 64, logprobs_wave_kernel<DT, 2>);
+    else GO(grid, per * 64, logprobs_wave_kernel<DT, 4>);
     return;
   }
   const long grid = rows < (1 << 20) ? rows : (1 << 20);
   // 16 waves per row where there are too few rows to fill the CUs with 4 (1 x 131072: 17.4 us against 22.8, 256 x 131072
   // 24.8 against 40.4); with more rows their phases cost more (512 x 131072 45.7 against 45.3, 333 x 50001 fp32 25.8
   // against 23.5, 1024 x 32768 47.6 against 25.2)
-  if (rows <= 256 && c >= 8192) GO((logprobs_kernel<DT, L, 16>), grid, 1024);
-  else GO((logprobs_kernel<DT, L, 4>), grid, 256);
+  if (rows <= 256 && c >= 8192) GO(grid, 1024, logprobs_kernel<DT, 16>);
+  else GO(grid, 256, logprobs_kernel<DT, 4>);
 #undef GO
 }
 
@@ -461,12 +536,9 @@ AI4E_API int ai4e_label_logprobs(const void* logits, long ld, long rows, int c, 
   if (rows == 0) return AI4E_OK;
   const Out out = {static_cast<float*>(logp), static_cast<float*>(entropy), static_cast<int*>(top_idx),
                    static_cast<float*>(top_logp)};
-#define GO(DT)                                                                                   \
-  if (wide) launch<DT, int64_t>(logits, ld, rows, c, labels, n_labels, k, out, s);               \
-  else launch<DT, int32_t>(logits, ld, rows, c, labels, n_labels, k, out, s)
-  if (dt == MX_BF16) { GO(MX_BF16); }
-  else if (dt == MX_F16) { GO(MX_F16); }
-  else { GO(MX_F32); }
-#undef GO
+  const Labels lab = {labels, n_labels, wide != 0};
+  if (dt == MX_BF16) launch<MX_BF16>(logits, ld, rows, c, lab, k, out, s);
+  else if (dt == MX_F16) launch<MX_F16>(logits, ld, rows, c, lab, k, out, s);
+  else launch<MX_F32>(logits, ld, rows, c, lab, k, out, s);
   return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
 }

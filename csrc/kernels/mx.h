@@ -37,14 +37,24 @@ struct mx_elem<MX_F32> {
   static __device__ __forceinline__ float from(float f) { return f; }
 };
 
-template <typename E>
-struct __attribute__((packed, aligned(sizeof(E)))) mx_pack8 {
-  E v[8];
+// Results go past L2 (non-temporal): they are read by a later kernel on any XCD, and would push inputs out of it (RMS norm
+// of 16384 x 8192 bf16: 196 us through L2, 173 past it). Inputs come through the caches, which often still hold what the
+// last kernel wrote (RMS norm of 1003 x 5000 fp32 15.0 us, with loads past them 20.6; of 16384 x 8192 bf16 181 and 179).
+typedef int mx_i32x4_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef int mx_i32x2_t __attribute__((ext_vector_type(2)));
+
+// as loaded: kept in whole registers until they are taken apart, so that a load can be in flight
+template <int DT>
+struct mx_raw8 {
+  mx_i32x4_t v[DT == MX_F32 ? 2 : 1];
 };
 
 template <int DT>
-__device__ __forceinline__ mx_pack8<typename mx_elem<DT>::type> mx_load8(const typename mx_elem<DT>::type* p) {
-  return *reinterpret_cast<const mx_pack8<typename mx_elem<DT>::type>*>(p);
+__device__ __forceinline__ mx_raw8<DT> mx_load8(const typename mx_elem<DT>::type* p) {
+  mx_raw8<DT> w;
+#pragma unroll
+  for (int i = 0; i < (DT == MX_F32 ? 2 : 1); ++i) w.v[i] = reinterpret_cast<const mx_i32x4_t*>(p)[i];
+  return w;
 }
 
 // the first n (0..8) of them, `fill` behind
@@ -55,15 +65,17 @@ __device__ __forceinline__ void mx_load8_tail(const typename mx_elem<DT>::type* 
 }
 
 template <int DT>
-__device__ __forceinline__ void mx_floats(const mx_pack8<typename mx_elem<DT>::type>& q, float (&f)[8]) {
+__device__ __forceinline__ void mx_floats(const mx_raw8<DT>& q, float (&f)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = mx_elem<DT>::one(q.v[i]);
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == MX_F32) {
+      f[i] = __int_as_float(q.v[0][i]);
+      f[4 + i] = __int_as_float(q.v[1][i]);
+    } else {
+      unpack2<DT == MX_F16>(static_cast<uint32_t>(q.v[0][i]), f[2 * i], f[2 * i + 1]);
+    }
+  }
 }
-
-// Results go past L2 (non-temporal): they are read by a later kernel on any XCD, and would push inputs out of it
-// (RMS norm of 16384 x 8192 bf16: 196 us through L2, 173 past it).
-typedef int mx_i32x4_t __attribute__((ext_vector_type(4), aligned(2)));
-typedef int mx_i32x2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ void mx_store_past(uint2* p, const uint2& v) {
   __builtin_nontemporal_store(mx_i32x2_t{static_cast<int>(v.x), static_cast<int>(v.y)}, reinterpret_cast<mx_i32x2_t*>(p));
@@ -73,8 +85,7 @@ __device__ __forceinline__ void mx_store_past(uint32_t* p, uint32_t v) { __built
 // 8 values, those below n
 template <int DT>
 __device__ __forceinline__ void mx_store8(typename mx_elem<DT>::type* p, const float (&f)[8], int n) {
-  typedef typename mx_elem<DT>::type E;
-  struct Pack { E v[8]; } q;
+  struct Pack { typename mx_elem<DT>::type v[8]; } q;
 #pragma unroll
   for (int i = 0; i < 8; ++i) q.v[i] = mx_elem<DT>::from(f[i]);
   if (n >= 8) {
