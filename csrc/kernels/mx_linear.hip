@@ -71,13 +71,16 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   constexpr int NW = WX * WW, BX = WX * TX * 32, BW = WW * TW * 32;
   typedef TileRow<FX> XR;
   typedef TileRow<MX_E2M1> WR;
-  constexpr int X_BYTES = BX * XR::BYTES, W_BYTES = BW * WR::BYTES, S_BYTES = (BX + BW) * 16;
+  // scales of x come for whole sets of 64 rows; SLOTS groups of 4 steps of them cover the stages ahead
+  constexpr int SX = (BX + 63) / 64 * 64, SLOTS = STAGES <= 4 ? 2 : 4;
+  constexpr int X_BYTES = BX * XR::BYTES, W_BYTES = BW * WR::BYTES, S_BYTES = (SX + BW) * 16;
   constexpr int STAGE = X_BYTES + W_BYTES, SCALES = STAGE * STAGES;
-  constexpr int X_DMA = X_BYTES / 1024 / NW, W_DMA = W_BYTES / 1024 / NW;
+  // DMAs per stage; the waves that a tile's DMAs do not divide among bring some twice
+  constexpr int X_ALL = X_BYTES / 1024, W_ALL = W_BYTES / 1024, S_ALL = S_BYTES / 1024;
+  constexpr int X_DMA = (X_ALL + NW - 1) / NW, W_DMA = (W_ALL + NW - 1) / NW, S_DMA = (S_ALL + NW - 1) / NW;
   constexpr int PER_STAGE = X_DMA + W_DMA;
-  constexpr int S_ALL = S_BYTES / 1024, S_DMA = (S_ALL + NW - 1) / NW;
-  static_assert(X_BYTES % (1024 * NW) == 0 && W_BYTES % (1024 * NW) == 0 && S_BYTES % 1024 == 0 && BX % 64 == 0, "");
-  static_assert(SCALES + 2 * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 4, "");
+  static_assert(X_BYTES % 1024 == 0 && W_BYTES % 1024 == 0 && S_BYTES % 1024 == 0, "");
+  static_assert(SCALES + SLOTS * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 8, "");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -93,19 +96,19 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   uint32_t xoff[X_DMA], woff[W_DMA];
 #pragma unroll
   for (int j = 0; j < X_DMA; ++j) {
-    const int row = (wave * X_DMA + j) * XR::PER_DMA + lane / XR::CHUNKS;
+    const int row = (wave * X_DMA + j) % X_ALL * XR::PER_DMA + lane / XR::CHUNKS;
     xoff[j] = static_cast<uint32_t>(min(row, m - 1 - x0)) * px + ((lane % XR::CHUNKS) ^ XR::swizzle(row)) * 16;
   }
 #pragma unroll
   for (int j = 0; j < W_DMA; ++j) {
-    const int row = (wave * W_DMA + j) * WR::PER_DMA + lane / WR::CHUNKS;
+    const int row = (wave * W_DMA + j) % W_ALL * WR::PER_DMA + lane / WR::CHUNKS;
     woff[j] = static_cast<uint32_t>(min(row, n - 1 - w0)) * pw + ((lane % WR::CHUNKS) ^ WR::swizzle(row)) * 16;
   }
-  uint32_t soff[S_DMA];  // a DMA brings the scales of 64 rows, first x's, then w's; the odd ones out bring some twice
+  uint32_t soff[S_DMA];  // a DMA brings the scales of 64 rows, first x's, then w's
 #pragma unroll
   for (int j = 0; j < S_DMA; ++j) {
     const int p = (wave + j * NW) % S_ALL;
-    soff[j] = static_cast<uint32_t>(p < BX / 64 ? min(p * 64 + lane, m - 1 - x0) : min(p * 64 - BX + lane, n - 1 - w0)) * ps;
+    soff[j] = static_cast<uint32_t>(p < SX / 64 ? min(p * 64 + lane, m - 1 - x0) : min(p * 64 - SX + lane, n - 1 - w0)) * ps;
   }
   const uint8_t* xb = x + static_cast<long>(x0) * px;
   const uint8_t* wb = w + static_cast<long>(w0) * pw;
@@ -113,6 +116,10 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   const uint8_t* wsb = ws + static_cast<long>(w0) * ps;
 
   const int nk = kp / MX_ALIGN;
+  // Where nobody else reads the same rows of w, each workgroup starts elsewhere along k: rows a power of two apart would
+  // else have all workgroups in the same memory channels at once (16 x 32768 x 8192 35 us, so 31). Whole groups of scales.
+  const int rot = tiles_x > 1 || nk % 4 ? 0 : w0 / BW * 5 * 4 % nk;
+  auto place = [&](int k) { return k + rot < nk ? k + rot : k + rot - nk; };
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
       (__attribute__((address_space(3))) uint8_t*)lds));
   // scales come 16 B of a row at a time, for 4 steps: as 4-B pieces they would be as many requests to L2 as the data
@@ -121,18 +128,18 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 #pragma unroll
     for (int j = 0; j < S_DMA; ++j) {
       const int p = (wave + j * NW) % S_ALL;
-      dma16((p < BX / 64 ? xsb : wsb) + static_cast<long>(min(4 * g, nk - 4)) * 4, soff[j],
-            lds0 + SCALES + (g & 1) * S_BYTES + p * 1024);
+      dma16((p < SX / 64 ? xsb : wsb) + static_cast<long>(place(min(4 * g, nk - 4))) * 4, soff[j],
+            lds0 + SCALES + (g & (SLOTS - 1)) * S_BYTES + p * 1024);
     }
   };
   // piece j of step kt; past the end the last step is brought again, into a slot that nobody reads
   auto issue = [&](int kt, uint32_t slot, int j) {
-    const int k = min(kt, nk - 1);
+    const int k = place(min(kt, nk - 1));
     const uint32_t base = lds0 + slot * STAGE;
     if (j < X_DMA)
-      dma16(xb + static_cast<long>(k) * XR::BYTES, xoff[j], base + (wave * X_DMA + j) * 1024);
+      dma16(xb + static_cast<long>(k) * XR::BYTES, xoff[j], base + (wave * X_DMA + j) % X_ALL * 1024);
     else
-      dma16(wb + static_cast<long>(k) * WR::BYTES, woff[j - X_DMA], base + X_BYTES + (wave * W_DMA + j - X_DMA) * 1024);
+      dma16(wb + static_cast<long>(k) * WR::BYTES, woff[j - X_DMA], base + X_BYTES + (wave * W_DMA + j - X_DMA) % W_ALL * 1024);
   };
 
   const int wx = wave % WX, ww = wave / WX;
@@ -165,11 +172,11 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   };
   // a row's four scale bytes of step kt, shifted so that bytes 0 and 2 are those of this half's blocks
   auto read_scales = [&](int kt, int(&ax)[TX], int(&aw)[TW]) {
-    const uint32_t st = lds0 + SCALES + ((kt >> 2) & 1) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4 + sa;
+    const uint32_t st = lds0 + SCALES + ((kt >> 2) & (SLOTS - 1)) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4 + sa;
 #pragma unroll
     for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<Lds4>(st + wx * TX * 512 + i * 512);
 #pragma unroll
-    for (int j = 0; j < TW; ++j) aw[j] = *reinterpret_cast<Lds4>(st + BX * 16 + ww * TW * 512 + j * 512);
+    for (int j = 0; j < TW; ++j) aw[j] = *reinterpret_cast<Lds4>(st + SX * 16 + ww * TW * 512 + j * 512);
   };
   auto shift_scales = [&]() {
 #pragma unroll
@@ -186,7 +193,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 
 #pragma unroll
   for (int s = 0; s < STAGES; ++s) {
-    if (s == 0) scales(0);
+    if (s % 4 == 0) scales(s / 4);
 #pragma unroll
     for (int j = 0; j < PER_STAGE; ++j) issue(s, s, j);
   }
@@ -280,7 +287,8 @@ template <int FX, int DT, int WX, int WW, int TX, int TW, int STAGES>
 int launch_tile(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
                 hipStream_t s) {
   constexpr int BX = WX * TX * 32, BW = WW * TW * 32;
-  constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES) + 2 * (BX + BW) * 16;
+  constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES) +
+                      (STAGES <= 4 ? 2 : 4) * ((BX + 63) / 64 * 64 + BW) * 16;
   const int tx = ai4e_cdiv(m, BX), tw = ai4e_cdiv(n, BW);
   auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES>;
   static const hipError_t ready =
@@ -385,31 +393,35 @@ int launch_slice(const void* x, const void* xs, const void* w, const void* ws, c
 }
 
 // Which kernel: the largest tile that still gives most of the 256 CUs one, since a larger tile moves fewer bytes per
-// product; where even 64 x 64 does not, slices of k, the smallest that need one round of workgroups. Measured at the
-// borders (us, e4m3, cold weights; the larger of each pair first):
+// product; where even 64 x 64 does not, the smallest slices of k or small tiles that need one round of workgroups.
+// Measured at the borders (us, e4m3, cold weights; the larger of each pair first):
 //   256 x 256 / 128 x 128   1024 x 8192 x 8192 (128 / 512 tiles) 77.7 / 61.8    4096 x 4096 x 4096 (256 / 1024) 55 / 70
 //   128 x 128 / 64 x 128    512 x 4096 x 4096 (128 / 256 tiles) 17.6 / 12.5     512 x 8192 x 8192 (256 / 512) 38.5 / 45.0
 //   64 x 128 / 64 x 64      256 x 4096 x 4096 (128 / 256 tiles) 12.1 / 11.1     256 x 8192 x 8192 (256 / 512) 26.4 / 33.0
-//   few rows, a large w: 16 x 32768 x 8192 128 x 128 42.0, 64 x 128 36.7, slices (1, 4) 38.1
-//   64 x 64 / slices        128 x 4096 x 4096 10.8 / 11.6 (2, 4)   64 x 4096 x 4096 10.7 / 9.0 (2, 2)   16 x 4096 x 4096 5.9 (1, 1)
+//   64 x 128 / 32 x 128     16 x 32768 x 8192 32.8 / 31.0     64 x 32768 x 8192 36.6 / 47.4
+//   64 x 64 / 32 x 64       64 x 8192 x 8192 (128 / 256 tiles) 21.3 / 17.8      200 x 3000 x 4096 (188 / 329) 11.2 / 14.1
+//   32 x 64 / slices        16 x 16384 x 8192 18.2 / 21.7 (1, 4)     16 x 8192 x 8192 16.9 / 10.4 (1, 2)
+//   64 x 64 / slices        64 x 4096 x 4096 10.7 / 9.0 (2, 2)       16 x 4096 x 4096 10.4 / 5.9 (1, 1)
 template <int FX, int DT>
 int launch(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
            hipStream_t s) {
 #define ARGS x, xs, w, ws, bias, m, n, kp, y, s
   const auto blocks = [&](int bm, int bn) { return static_cast<long>(ai4e_cdiv(m, bm)) * ai4e_cdiv(n, bn); };
   constexpr long FILL = 192, ROUND = 320;
-  if (kp >= 512) {  // the tiles' scales come four steps of 128 at a time
-    if (m > 128 && blocks(256, 256) >= FILL)
-      return launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(ARGS);
-    if (m > 64 && blocks(128, 128) >= FILL)
-      return launch_tile<FX, DT, 2, 2, 2, 2, FX == MX_E4M3 ? 3 : 4>(ARGS);
-    if (blocks(64, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 2, 4>(ARGS);
+  const bool tiles = kp >= 512;  // their scales come four steps of 128 at a time
+  if (tiles) {
+    if (m > 128 && blocks(256, 256) >= FILL) return launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(ARGS);
+    if (m > 64 && blocks(128, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 2, 2, FX == MX_E4M3 ? 3 : 4>(ARGS);
+    if (m <= 32 && blocks(32, 128) >= FILL) return launch_tile<FX, DT, 1, 4, 1, 1, 4>(ARGS);
+    if (m > 32 && blocks(64, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 2, 4>(ARGS);
+    if (m > 32 && blocks(64, 64) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
   }
   if (blocks(16, 16) <= ROUND) return launch_slice<FX, DT, 1, 1>(ARGS);
   if (blocks(16, 32) <= ROUND) return launch_slice<FX, DT, 1, 2>(ARGS);
+  if (tiles && blocks(32, 64) >= FILL && blocks(32, 64) <= ROUND) return launch_tile<FX, DT, 1, 2, 1, 1, 8>(ARGS);
   if (m <= 16) return launch_slice<FX, DT, 1, 4>(ARGS);
   if (blocks(32, 32) <= ROUND) return launch_slice<FX, DT, 2, 2>(ARGS);
-  return kp >= 512 ? launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS) : launch_slice<FX, DT, 2, 4>(ARGS);
+  return tiles ? launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS) : launch_slice<FX, DT, 2, 4>(ARGS);
 #undef ARGS
 }
 

@@ -118,9 +118,10 @@ def test_linear_large(m, n, k, fmt):
 @pytest.mark.parametrize("fmt,dtype", [("e4m3", torch.bfloat16), ("e4m3", torch.float16), ("e2m1", torch.bfloat16),
                                        ("e2m1", torch.float32)])
 @pytest.mark.parametrize("m,n,k", [(70, 12500, 1000), (1600, 2001, 640), (3500, 3699, 520), (2500, 300, 200),
-                                   (3300, 4100, 1664)])
+                                   (3300, 4100, 1664), (20, 24601, 1024), (32, 24600, 640), (70, 4201, 1024),
+                                   (128, 4096, 1536), (16, 14000, 512), (64, 12300, 2048)])
 def test_linear_every_tile(m, n, k, fmt, dtype):
-    """64 x 128, 128 x 128 and 256 x 256 tiles, slices of many rows, odd counts of steps."""
+    """Every tile kernel, slices of many rows, odd counts of steps."""
     check_linear(m, n, k, fmt, dtype, bias=True, seed=m)
 
 
