@@ -71,8 +71,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   constexpr int NW = WX * WW, BX = WX * TX * 32, BW = WW * TW * 32;
   typedef TileRow<FX> XR;
   typedef TileRow<MX_E2M1> WR;
-  // scales of x come for whole sets of 64 rows; SLOTS groups of 4 steps of them cover the stages ahead
-  constexpr int SX = (BX + 63) / 64 * 64, SLOTS = STAGES <= 4 ? 2 : 4;
+  constexpr int SX = (BX + 63) / 64 * 64;  // scales of x come for whole sets of 64 rows
   constexpr int X_BYTES = BX * XR::BYTES, W_BYTES = BW * WR::BYTES, S_BYTES = (SX + BW) * 16;
   constexpr int STAGE = X_BYTES + W_BYTES, SCALES = STAGE * STAGES;
   // DMAs per stage; the waves that a tile's DMAs do not divide among bring some twice
@@ -80,7 +79,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   constexpr int X_DMA = (X_ALL + NW - 1) / NW, W_DMA = (W_ALL + NW - 1) / NW, S_DMA = (S_ALL + NW - 1) / NW;
   constexpr int PER_STAGE = X_DMA + W_DMA;
   static_assert(X_BYTES % 1024 == 0 && W_BYTES % 1024 == 0 && S_BYTES % 1024 == 0, "");
-  static_assert(SCALES + SLOTS * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 8, "");
+  static_assert(SCALES + 2 * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 4, "");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     for (int j = 0; j < S_DMA; ++j) {
       const int p = (wave + j * NW) % S_ALL;
       dma16((p < SX / 64 ? xsb : wsb) + static_cast<long>(place(min(4 * g, nk - 4))) * 4, soff[j],
-            lds0 + SCALES + (g & (SLOTS - 1)) * S_BYTES + p * 1024);
+            lds0 + SCALES + (g & 1) * S_BYTES + p * 1024);
     }
   };
   // piece j of step kt; past the end the last step is brought again, into a slot that nobody reads
@@ -172,7 +171,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   };
   // a row's four scale bytes of step kt, shifted so that bytes 0 and 2 are those of this half's blocks
   auto read_scales = [&](int kt, int(&ax)[TX], int(&aw)[TW]) {
-    const uint32_t st = lds0 + SCALES + ((kt >> 2) & (SLOTS - 1)) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4 + sa;
+    const uint32_t st = lds0 + SCALES + ((kt >> 2) & 1) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4 + sa;
 #pragma unroll
     for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<Lds4>(st + wx * TX * 512 + i * 512);
 #pragma unroll
@@ -193,7 +192,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 
 #pragma unroll
   for (int s = 0; s < STAGES; ++s) {
-    if (s % 4 == 0) scales(s / 4);
+    if (s == 0) scales(0);
 #pragma unroll
     for (int j = 0; j < PER_STAGE; ++j) issue(s, s, j);
   }
@@ -288,7 +287,7 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
                 hipStream_t s) {
   constexpr int BX = WX * TX * 32, BW = WW * TW * 32;
   constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES) +
-                      (STAGES <= 4 ? 2 : 4) * ((BX + 63) / 64 * 64 + BW) * 16;
+                      2 * ((BX + 63) / 64 * 64 + BW) * 16;
   const int tx = ai4e_cdiv(m, BX), tw = ai4e_cdiv(n, BW);
   auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES>;
   static const hipError_t ready =
@@ -300,11 +299,11 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
   return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
 }
 
-// The slice kernel: 16 MT rows of x by 16 NT rows of w per workgroup, k cut over its 8 waves: for outputs too few to give
-// every CU a tile, where latency counts. Operands go from memory to registers, in steps of
-// v_mfma_scale_f32_16x16x128: lane l holds row l & 15, k = 32 (l >> 4) .. + 31 of e2m1, 16 (l >> 4) .. + 15 and
-// 64 + 16 (l >> 4) .. + 15 of e4m3, the scale of block l >> 4; of D column l & 15, rows 4 (l >> 4) + i. Four steps' loads go
-// out together, their scales as one 16-B load per row. The waves' sums are added in LDS, always in the same order.
+// The slice kernel: 16 MT rows of x by 16 NT rows of w per workgroup, k cut over its 8 waves: for the fewest rows, where
+// latency counts, and for k below 512. Operands go from memory to registers, in steps of v_mfma_scale_f32_16x16x128: lane l
+// holds row l & 15, k = 32 (l >> 4) .. + 31 of e2m1, 16 (l >> 4) .. + 15 and 64 + 16 (l >> 4) .. + 15 of e4m3, the scale
+// of block l >> 4; of D column l & 15, rows 4 (l >> 4) + i. Four steps' loads go out together, their scales as one 16-B
+// load per row. The waves' sums are added in LDS, always in the same order.
 constexpr int SLICES = 8;
 
 template <int FX, int DT, int MT, int NT>
@@ -392,36 +391,185 @@ int launch_slice(const void* x, const void* xs, const void* w, const void* ws, c
   return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
 }
 
+// The stream kernel: 32 rows of x by 32 TW rows of w per workgroup, k cut over its 4 waves, each of which runs its steps
+// through a ring of its own in LDS: no barrier until the waves' sums are added, always in the same order. For outputs
+// too few to give every CU a tile of 64 x 64, whose single workgroup would wait out every step's latency (333 x 5000 x
+// 1000: 12.9 us, so 8.2).
+constexpr int STREAMS = 4;
+
+template <int FX, int TW, int STAGES>
+struct StreamLds {
+  static constexpr int X_BYTES = 32 * TileRow<FX>::BYTES, W_BYTES = 32 * TW * TileRow<MX_E2M1>::BYTES;
+  static constexpr int S_ROWS = (32 + 32 * TW + 63) / 64 * 64, S_BYTES = S_ROWS * 16;  // 4 steps' scales: x's rows, w's
+  static constexpr int STAGE = X_BYTES + W_BYTES, SCALES = STAGES * STAGE, WAVE = SCALES + 2 * S_BYTES;
+  static constexpr int SUMS = STREAMS * TW * 16 * 64 * 4;
+  static constexpr int ALL = STREAMS * WAVE > SUMS ? STREAMS * WAVE : SUMS;
+  static_assert(STAGES >= 2 && STAGES <= 4 && ALL <= 160 * 1024 && WAVE % 128 == 0, "");
+};
+
+template <int FX, int DT, int TW, int STAGES>
+__global__ __launch_bounds__(STREAMS * 64) void mx_stream_kernel(
+    const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w,
+    const uint8_t* __restrict__ ws, const float* __restrict__ bias, int m, int n, int kp, int tiles_x,
+    typename mx_elem<DT>::type* __restrict__ y) {
+  typedef TileRow<FX> XR;
+  typedef TileRow<MX_E2M1> WR;
+  typedef StreamLds<FX, TW, STAGES> S;
+  constexpr int BW = TW * 32, S_DMA = S::S_ROWS / 64, X_DMA = S::X_BYTES / 1024, W_DMA = S::W_BYTES / 1024;
+  constexpr int PER_STAGE = X_DMA + W_DMA;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, half = lane >> 5, r = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = xcd_remap(blockIdx.x, gridDim.x);  // the row blocks of one w block follow each other: its L2 serves them
+  const int x0 = t % tiles_x * 32, w0 = t / tiles_x * BW;
+  const int px = FX == MX_E4M3 ? kp : kp / 2, pw = kp / 2, ps = kp / 32;
+  uint32_t xoff[X_DMA], woff[W_DMA];
+#pragma unroll
+  for (int j = 0; j < X_DMA; ++j) {
+    const int row = j * XR::PER_DMA + lane / XR::CHUNKS;
+    xoff[j] = static_cast<uint32_t>(min(row, m - 1 - x0)) * px + ((lane % XR::CHUNKS) ^ XR::swizzle(row)) * 16;
+  }
+#pragma unroll
+  for (int j = 0; j < W_DMA; ++j) {
+    const int row = j * WR::PER_DMA + lane / WR::CHUNKS;
+    woff[j] = static_cast<uint32_t>(min(row, n - 1 - w0)) * pw + ((lane % WR::CHUNKS) ^ WR::swizzle(row)) * 16;
+  }
+  const uint8_t* xb = x + static_cast<long>(x0) * px;
+  const uint8_t* wb = w + static_cast<long>(w0) * pw;
+  const uint8_t* sp[S_DMA];
+#pragma unroll
+  for (int j = 0; j < S_DMA; ++j) {
+    const int p = j * 64 + lane;
+    sp[j] = p < 32 ? xs + static_cast<long>(min(x0 + p, m - 1)) * ps
+                   : ws + static_cast<long>(min(w0 + min(p - 32, BW - 1), n - 1)) * ps;
+  }
+  // whole groups of 4 steps per wave; the last group's scales end with the row
+  const int nk = kp / MX_ALIGN, groups = (nk + 3) / 4;
+  const int k0 = groups * wave / STREAMS * 4, k1 = min(groups * (wave + 1) / STREAMS * 4, nk);
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) uint8_t*)lds)) + wave * S::WAVE;
+  // step kt into a slot; past the wave's end its last step is brought again, into a slot that nobody reads
+  auto issue = [&](int kt, uint32_t slot) {
+    const int k = __builtin_amdgcn_readfirstlane(min(kt, k1 - 1));
+    const uint32_t base = lds0 + slot * S::STAGE;
+    if ((kt & 3) == 0) {
+      const long at = min(k & ~3, nk - 4) * 4l;
+#pragma unroll
+      for (int j = 0; j < S_DMA; ++j)
+        ai4e_conv::glds16(sp[j] + at, lds0 + S::SCALES + ((kt >> 2) & 1) * S::S_BYTES + j * 1024);
+    }
+#pragma unroll
+    for (int j = 0; j < X_DMA; ++j) dma16(xb + static_cast<long>(k) * XR::BYTES, xoff[j], base + j * 1024);
+#pragma unroll
+    for (int j = 0; j < W_DMA; ++j) dma16(wb + static_cast<long>(k) * WR::BYTES, woff[j], base + S::X_BYTES + j * 1024);
+  };
+  const uint32_t xa = r * XR::BYTES + (half ^ XR::swizzle(r)) * 16;
+  const uint32_t wa = S::X_BYTES + r * WR::BYTES + (half ^ WR::swizzle(r)) * 16;
+  typedef __attribute__((address_space(3))) const i32x4_t* Lds16;
+  typedef __attribute__((address_space(3))) const int* Lds4;
+  f32x16_t acc[TW] = {};
+  if (k0 < k1) {
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) issue(k0 + s, s);
+    uint32_t slot = 0;
+    for (int kt = k0; kt < k1; ++kt) {
+      ai4e_conv::wait_vmcnt<(STAGES - 1) * PER_STAGE>();  // step kt is there, and its scales, which went out before it
+      const uint32_t st = lds0 + slot * S::STAGE;
+      const uint32_t sa = lds0 + S::SCALES + ((kt >> 2) & 1) * S::S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4 + r * 16;
+      i32x8_t fx[2], fw[2][TW];
+      int sw[TW];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if constexpr (FX == MX_E4M3) {
+          const i32x4_t a = *reinterpret_cast<Lds16>((st + xa) ^ (64 * u));
+          const i32x4_t b = *reinterpret_cast<Lds16>((st + xa) ^ (64 * u + 32));
+          fx[u] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+          const i32x4_t a = *reinterpret_cast<Lds16>((st + xa) ^ (32 * u));
+          fx[u] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+#pragma unroll
+        for (int j = 0; j < TW; ++j) {
+          const i32x4_t a = *reinterpret_cast<Lds16>(((st + wa) ^ (32 * u)) + j * 32 * WR::BYTES);
+          fw[u][j] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+      }
+      const int sx = *reinterpret_cast<Lds4>(sa) >> (8 * half);
+#pragma unroll
+      for (int j = 0; j < TW; ++j) sw[j] = *reinterpret_cast<Lds4>(sa + (1 + j) * 512) >> (8 * half);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
+      issue(kt + STAGES, slot);
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+#pragma unroll
+      for (int j = 0; j < TW; ++j)
+        acc[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[0][j], fx[0], acc[j], 4, FX == MX_E4M3 ? 0 : 4, 0,
+                                                                 sw[j], 0, sx);
+#pragma unroll
+      for (int j = 0; j < TW; ++j)
+        acc[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[1][j], fx[1], acc[j], 4, FX == MX_E4M3 ? 0 : 4, 2,
+                                                                 sw[j], 2, sx);
+    }
+    ai4e_conv::wait_vmcnt<0>();
+  }
+  __syncthreads();  // every wave is through with its ring
+  f32x4_t* part = reinterpret_cast<f32x4_t*>(lds);  // [wave][TW][4][lane]
+#pragma unroll
+  for (int j = 0; j < TW; ++j)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      part[((wave * TW + j) * 4 + q) * 64 + lane] =
+          f32x4_t{acc[j][4 * q], acc[j][4 * q + 1], acc[j][4 * q + 2], acc[j][4 * q + 3]};
+  __syncthreads();
+  for (int f = wave; f < TW * 4; f += STREAMS) {
+    f32x4_t v = part[f * 64 + lane];
+#pragma unroll
+    for (int p = 1; p < STREAMS; ++p) v += part[(p * TW * 4 + f) * 64 + lane];
+    const int row = x0 + r;
+    if (row < m) store4<DT>(y + static_cast<long>(row) * n, w0 + f / 4 * 32 + 8 * (f % 4) + 4 * half, n, bias, v);
+  }
+}
+
+template <int FX, int DT, int TW, int STAGES>
+int launch_stream(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
+                  hipStream_t s) {
+  constexpr int LDS = StreamLds<FX, TW, STAGES>::ALL;
+  const int tx = ai4e_cdiv(m, 32), tw = ai4e_cdiv(n, 32 * TW);
+  auto* kernel = mx_stream_kernel<FX, DT, TW, STAGES>;
+  static const hipError_t ready =
+      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  if (ready != hipSuccess) return AI4E_ELAUNCH;
+  hipLaunchKernelGGL(kernel, dim3(tx * tw), dim3(STREAMS * 64), LDS, s, static_cast<const uint8_t*>(x),
+                     static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(ws),
+                     static_cast<const float*>(bias), m, n, kp, tx, static_cast<typename mx_elem<DT>::type*>(y));
+  return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
+}
+
 // Which kernel: the largest tile that still gives most of the 256 CUs one, since a larger tile moves fewer bytes per
-// product; where even 64 x 64 does not, the smallest slices of k or small tiles that need one round of workgroups.
-// Measured at the borders (us, e4m3, cold weights; the larger of each pair first):
+// product; where even 64 x 64 does not, the streams that need one round of workgroups, and for the fewest rows slices.
+// Measured at the borders (us, e4m3, cold weights; the first kernel's time first):
 //   256 x 256 / 128 x 128   1024 x 8192 x 8192 (128 / 512 tiles) 77.7 / 61.8    4096 x 4096 x 4096 (256 / 1024) 55 / 70
 //   128 x 128 / 64 x 128    512 x 4096 x 4096 (128 / 256 tiles) 17.6 / 12.5     512 x 8192 x 8192 (256 / 512) 38.5 / 45.0
-//   64 x 128 / 64 x 64      256 x 4096 x 4096 (128 / 256 tiles) 12.1 / 11.1     256 x 8192 x 8192 (256 / 512) 26.4 / 33.0
-//   64 x 128 / 32 x 128     16 x 32768 x 8192 32.8 / 31.0     64 x 32768 x 8192 36.6 / 47.4
-//   64 x 64 / 32 x 64       64 x 8192 x 8192 (128 / 256 tiles) 21.3 / 17.8      200 x 3000 x 4096 (188 / 329) 11.2 / 14.1
-//   32 x 64 / slices        16 x 16384 x 8192 18.2 / 21.7 (1, 4)     16 x 8192 x 8192 16.9 / 10.4 (1, 2)
-//   64 x 64 / slices        64 x 4096 x 4096 10.7 / 9.0 (2, 2)       16 x 4096 x 4096 10.4 / 5.9 (1, 1)
+//   64 x 128 / 64 x 64      256 x 4096 x 4096 (128 / 256 tiles) 12.5 / 10.9     256 x 8192 x 8192 (256 / 512) 26.4 / 33.0
+//   64 x 64 / stream 2      128 x 4096 x 4096 (128 / 256) 10.6 / 7.8            200 x 3000 x 4096 (188 / 329) 11.0 / 11.4
+//   32 x 128 / stream 2     16 x 24576 x 4096 (192 / 384) 15.7 / 18.3           16 x 16384 x 4096 (128 / 256) 14.2 / 11.0
+//   stream 2 / stream 1     64 x 6144 x 4096 (192 / 384) 9.6 / 11.4             64 x 4096 x 4096 (128 / 256) 7.3 / 6.1
+//   stream 1 / slices       1 x 4096 x 4096 5.6 / 4.4                           16 x 4096 x 4096 5.7 / 5.9
 template <int FX, int DT>
 int launch(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
            hipStream_t s) {
 #define ARGS x, xs, w, ws, bias, m, n, kp, y, s
   const auto blocks = [&](int bm, int bn) { return static_cast<long>(ai4e_cdiv(m, bm)) * ai4e_cdiv(n, bn); };
   constexpr long FILL = 192, ROUND = 320;
-  const bool tiles = kp >= 512;  // their scales come four steps of 128 at a time
-  if (tiles) {
-    if (m > 128 && blocks(256, 256) >= FILL) return launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(ARGS);
-    if (m > 64 && blocks(128, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 2, 2, FX == MX_E4M3 ? 3 : 4>(ARGS);
-    if (m <= 32 && blocks(32, 128) >= FILL) return launch_tile<FX, DT, 1, 4, 1, 1, 4>(ARGS);
-    if (m > 32 && blocks(64, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 2, 4>(ARGS);
-    if (m > 32 && blocks(64, 64) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
-  }
-  if (blocks(16, 16) <= ROUND) return launch_slice<FX, DT, 1, 1>(ARGS);
-  if (blocks(16, 32) <= ROUND) return launch_slice<FX, DT, 1, 2>(ARGS);
-  if (tiles && blocks(32, 64) >= FILL && blocks(32, 64) <= ROUND) return launch_tile<FX, DT, 1, 2, 1, 1, 8>(ARGS);
-  if (m <= 16) return launch_slice<FX, DT, 1, 4>(ARGS);
-  if (blocks(32, 32) <= ROUND) return launch_slice<FX, DT, 2, 2>(ARGS);
-  return tiles ? launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS) : launch_slice<FX, DT, 2, 4>(ARGS);
+  if (kp < 512)  // the others' scales come four steps of 128 at a time
+    return blocks(16, 16) <= ROUND ? launch_slice<FX, DT, 1, 1>(ARGS) : launch_slice<FX, DT, 2, 4>(ARGS);
+  if (m <= 8 && blocks(16, 16) <= ROUND) return launch_slice<FX, DT, 1, 1>(ARGS);
+  if (m > 128 && blocks(256, 256) >= FILL) return launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(ARGS);
+  if (m > 64 && blocks(128, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 2, 2, FX == MX_E4M3 ? 3 : 4>(ARGS);
+  if (m > 32 && blocks(64, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 2, 4>(ARGS);
+  if (m > 32 && blocks(64, 64) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
+  if (blocks(32, 32) <= ROUND) return launch_stream<FX, DT, 1, 2>(ARGS);
+  if (blocks(32, 64) <= ROUND) return launch_stream<FX, DT, 2, 2>(ARGS);
+  return m <= 32 ? launch_tile<FX, DT, 1, 4, 1, 1, 4>(ARGS) : launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
 #undef ARGS
 }
 
