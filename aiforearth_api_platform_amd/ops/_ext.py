@@ -81,6 +81,7 @@ _SIGS = {
     "ai4e_label_logprobs": [_vp, _c_long, _c_long, _c_int, _c_int, _vp, _c_int, _c_int, _c_int] + [_vp] * 5,
     "ai4e_crumbs_alloc": [_c_int, _vp, _vp],
     "ai4e_crumb": [_vp, _c_int, _vp],
+    "ai4e_clear_error": [],
 }
 
 

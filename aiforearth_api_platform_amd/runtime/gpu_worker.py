@@ -102,12 +102,19 @@ def ring_jpeg_key(shm, nslots: int, item_shape: Sequence[int]) -> int:
 
 
 def pin_host(buf: torch.Tensor) -> bool:
-    """Register the mapped ring as pinned host memory for direct DMA (hipHostRegister)."""
+    """Register the mapped ring as pinned host memory for direct DMA (hipHostRegister). A system may refuse that; batches
+    are then copied from pageable memory, and the error must not surface in the next GPU call."""
     try:
         rc = torch.cuda.cudart().cudaHostRegister(buf.data_ptr(), buf.numel(), 0)
-        return (int(rc[0]) if isinstance(rc, tuple) else int(rc)) == 0
+        if (int(rc[0]) if isinstance(rc, tuple) else int(rc)) == 0:
+            return True
     except Exception:
-        return False
+        pass
+    from ..ops import _ext
+
+    if _ext.available():
+        _ext.call_int("ai4e_clear_error")
+    return False
 
 
 class _Pending:

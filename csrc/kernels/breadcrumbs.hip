@@ -33,6 +33,9 @@ AI4E_API int ai4e_crumbs_alloc(int n, void* host_out, void* dev_out) {
   return AI4E_OK;
 }
 
+// the error that a refused runtime call left for the next one to report (0: none), cleared
+AI4E_API int ai4e_clear_error() { return static_cast<int>(hipGetLastError()); }
+
 AI4E_API int ai4e_crumb(void* dev, int idx, hipStream_t s) {
   hipLaunchKernelGGL(crumb_kernel, dim3(1), dim3(64), 0, s, static_cast<int*>(dev), idx);
   return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
