@@ -6,16 +6,15 @@
 // in, 2 B (h) and 1.03 B (codes, scales) out for 16-bit rows. A workgroup per row, or for narrow rows the 16, 32 or 64
 // lanes that its chunks of 8 fill.
 // A value next to the border of two 8-bit neighbours falls to either side by the last bit of y, so y is computed to
-// one rounding: the row's factor as a double, split into a float and its remainder, and h * factor with its error. Where
+// one rounding: squares and the row's factor in double, the factor split into a float and its remainder, and h * factor with its error. Where
 // that rounding ends on a border it is taken back by a bit towards y, so that the 8-bit rounding sees y's side of it.
 #include "mx.h"
 
 namespace {
 
-// sum over a row's LANES lanes of a per-lane float (a lane's own sum has at most a row's share of squares), in double
+// sum over a row's LANES lanes
 template <int LANES>
-__device__ __forceinline__ double row_sum(float v, double* lds) {
-  double s = v;
+__device__ __forceinline__ double row_sum(double s, double* lds) {
 #pragma unroll
   for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if constexpr (LANES > 64) {
@@ -74,36 +73,17 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_mx8_kernel
     const auto* xr = x + row * ldx;
     const auto* rr = res ? res + row * ldr : nullptr;
     float h[KEEP][8];
-    float sq = 0.f;
+    double sq = 0;  // in 64 bits, which the unit adds at the same rate: no square leaves its range
 #pragma unroll
     for (int j = 0; j < nch; ++j) {
       const int col = (j * LANES + tid) * 8;
       float(&v)[8] = h[CH > 0 ? j : 0];
       load_h<DT>(xr + col, rr ? rr + col : nullptr, c - col, v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sq = fmaf(v[i], v[i], sq);
+      for (int i = 0; i < 8; ++i) sq = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), sq);
       if (hout) mx_store8_quad<DT>(hout + row * c, col, c, v);
     }
-    double ms = row_sum<LANES>(sq, lds);
-    double factor;
-    if (ms < 3e38) {
-      factor = inv_sqrt(ms * inv_c + static_cast<double>(eps));
-    } else {  // the squares left 32 bits (or are not finite): once more, scaled by 2^-80
-      sq = 0.f;
-#pragma unroll
-      for (int j = 0; j < nch; ++j) {
-        const int col = (j * LANES + tid) * 8;
-        float(&v)[8] = h[CH > 0 ? j : 0];
-        if (CH == 0) load_h<DT>(xr + col, rr ? rr + col : nullptr, c - col, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float u = v[i] * 0x1p-80f;
-          sq = fmaf(u, u, sq);
-        }
-      }
-      ms = row_sum<LANES>(sq, lds);
-      factor = 1.0 / (sqrt(ms * inv_c + static_cast<double>(eps) * 0x1p-160) * 0x1p80);
-    }
+    const double factor = inv_sqrt(row_sum<LANES>(sq, lds) * inv_c + static_cast<double>(eps));
     const float fh = static_cast<float>(factor), fl = static_cast<float>(factor - static_cast<double>(fh));
 #pragma unroll
     for (int j = 0; j < nch; ++j) {
