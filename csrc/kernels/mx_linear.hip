@@ -9,6 +9,7 @@
 //   of D it holds column l & 31 (a row of x), rows 8 (i >> 2) + 4 (l >> 5) + (i & 3), i = 0..15 (rows of w)
 // Operands of registers alone run at 4.4 PFLOP/s with e4m3 on one side and 8.0 with e2m1 on both, whose 32 x 32 x 64
 // form is twice as fast as the 16 x 16 x 128 one; hence the large tiles are made of it.
+#include <atomic>
 #include <type_traits>
 
 #include "conv_common.h"
@@ -33,6 +34,17 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t l
       : "=&s"(keep)
       : "v"(off), "s"(base), "s"(lds)
       : "memory");
+}
+
+// Dynamic LDS over 64 KB is allowed per kernel and device, before its first launch there. `devices`: where it is.
+bool allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>& devices) {
+  int d = 0;
+  if (hipGetDevice(&d) != hipSuccess) return false;
+  const uint64_t bit = 1ull << (d & 63);
+  if (devices.load(std::memory_order_acquire) & bit) return true;
+  if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+  devices.fetch_or(bit, std::memory_order_release);
+  return true;
 }
 
 // four consecutive outputs of a row, those below n
@@ -290,9 +302,8 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
                       2 * ((BX + 63) / 64 * 64 + BW) * 16;
   const int tx = ai4e_cdiv(m, BX), tw = ai4e_cdiv(n, BW);
   auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES>;
-  static const hipError_t ready =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-  if (ready != hipSuccess) return AI4E_ELAUNCH;
+  static std::atomic<uint64_t> devices{0};
+  if (!allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices)) return AI4E_ELAUNCH;
   hipLaunchKernelGGL(kernel, dim3(tx * tw), dim3(WX * WW * 64), LDS, s, static_cast<const uint8_t*>(x),
                      static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(ws),
                      static_cast<const float*>(bias), m, n, kp, tx, tw, static_cast<typename mx_elem<DT>::type*>(y));
@@ -535,9 +546,8 @@ int launch_stream(const void* x, const void* xs, const void* w, const void* ws, 
   constexpr int LDS = StreamLds<FX, TW, STAGES>::ALL;
   const int tx = ai4e_cdiv(m, 32), tw = ai4e_cdiv(n, 32 * TW);
   auto* kernel = mx_stream_kernel<FX, DT, TW, STAGES>;
-  static const hipError_t ready =
-      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-  if (ready != hipSuccess) return AI4E_ELAUNCH;
+  static std::atomic<uint64_t> devices{0};
+  if (!allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices)) return AI4E_ELAUNCH;
   hipLaunchKernelGGL(kernel, dim3(tx * tw), dim3(STREAMS * 64), LDS, s, static_cast<const uint8_t*>(x),
                      static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(ws),
                      static_cast<const float*>(bias), m, n, kp, tx, static_cast<typename mx_elem<DT>::type*>(y));

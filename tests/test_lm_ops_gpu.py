@@ -1,6 +1,9 @@
 """Language-model operators on the GPU against 64-bit oracles: MX quantisation, MX product, RMS norm to e4m3, label
 log-probabilities; then the four in a row, on streams and in graphs."""
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -403,6 +406,40 @@ def test_two_captured_graphs(rows):
         for o, w, s in zip(outs, want, sets):
             assert all(torch.equal(a, b) for a, b in zip(o, w)), turn
             assert all(torch.equal(a, b) for a, b in zip(tail(*s), w))
+
+
+FIRST_CALL = """
+import torch
+from aiforearth_api_platform_amd.ops.head import label_logprobs
+from aiforearth_api_platform_amd.ops.mx import mx_linear, mx_quantize, mx_dequantize
+from aiforearth_api_platform_amd.ops.norm import rms_norm_mx8
+x, w = torch.randn(300, 640, device="cuda"), torch.randn(4100, 640, device="cuda")
+gamma, labels = torch.ones(640, device="cuda"), torch.arange(300, device="cuda")
+
+def run(rows):
+    q, h = rms_norm_mx8(x[:rows], gamma, x[:rows])
+    y = mx_linear(q, mx_quantize(w))
+    return [h, y, mx_dequantize(q), *label_logprobs(y, labels[:rows], 3)]
+
+rows = (1, 16, 60, 300)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    outs = [run(r) for r in rows]
+for _ in range(3):
+    g.replay()
+    torch.cuda.synchronize()
+    for r, out in zip(rows, outs):
+        assert all(torch.equal(a, b) for a, b in zip(out, run(r))), r
+print("same")
+"""
+
+
+def test_first_calls_in_a_capture():
+    """A process whose first calls of the operators are captured: nothing is set up at a first eager call."""
+    root = Path(__file__).resolve().parent.parent
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "same" in r.stdout, r.stdout + r.stderr[-2000:]
 
 
 def test_gpu_refusals():
