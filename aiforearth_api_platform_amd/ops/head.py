@@ -47,8 +47,8 @@ def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, 
     -inf and entropy 0. A row with a NaN or +inf has no distribution: NaN, classes -1. A negative label means that the
     row has none: 0, so that sums pass over it; one of C or more gives NaN. No backward pass."""
     c = logits.shape[-1] if logits.dim() else 0
-    if logits.dtype not in mx.DTYPE_CODE or c == 0:
-        raise ValueError("label_logprobs expects bfloat16, float16 or float32 logits of at least one class")
+    if logits.dtype not in mx.DTYPE_CODE or not 0 < c <= mx.MAX_WIDTH:
+        raise ValueError("label_logprobs expects bfloat16, float16 or float32 logits of 1 to 2^30 classes")
     if not 0 <= k <= min(c, MAX_ALTERNATIVES):
         raise ValueError(f"label_logprobs: k is 0 to {min(c, MAX_ALTERNATIVES)}, not {k}")
     lead, index = logits.shape[:-1], logits.get_device()

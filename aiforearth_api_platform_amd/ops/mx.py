@@ -19,6 +19,7 @@ import torch.nn.functional as F
 from . import _ext
 
 BLOCK, ALIGN = 32, 128
+MAX_WIDTH = 1 << 30  # values of a row, here and where a row of logits or of a norm is taken
 DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # element types at the C entries (csrc/kernels/mx.h)
 FMT_CODE = {"e4m3": 0, "e2m1": 1}
 _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
@@ -62,13 +63,15 @@ def empty(lead, k: int, fmt: str, device) -> MxTensor:
 
 
 def check(name: str, q: MxTensor) -> None:
-    """Raises ValueError unless ``q`` has the layout that MxTensor describes."""
+    """Raises TypeError or ValueError unless ``q`` has the layout that MxTensor describes."""
+    if not isinstance(q, MxTensor):
+        raise TypeError(f"{name}: an MxTensor is expected, not {type(q).__name__}")
     data, scale, k = q
     e2m1 = data.dtype == torch.uint8
     if not (e2m1 or data.dtype == torch.float8_e4m3fn) or scale.dtype not in (torch.uint8, torch.float8_e8m0fnu):
         raise ValueError(f"{name}: data is uint8 (e2m1) or float8_e4m3fn, scale float8_e8m0fnu or uint8")
     kp, shape, scales = padded(k), data.shape, scale.shape
-    if (k <= 0 or len(shape) < 1 or len(scales) < 1 or scales[-1] * BLOCK != kp or shape[-1] != (kp // 2 if e2m1 else kp)
+    if (not 0 < k <= MAX_WIDTH or len(shape) < 1 or len(scales) < 1 or scales[-1] * BLOCK != kp or shape[-1] != (kp // 2 if e2m1 else kp)
             or shape[:-1] != scales[:-1]):
         raise ValueError(f"{name}: data {tuple(shape)} and scale {tuple(scales)} do not hold rows of {k}")
     if data.get_device() != scale.get_device() or not data.is_contiguous() or not scale.is_contiguous():
@@ -123,8 +126,8 @@ def mx_quantize(x: torch.Tensor, fmt: str = "e2m1") -> MxTensor:
     """``[..., K]`` (bf16, fp16 or fp32; rows may be strided) -> MxTensor of ``fmt`` ("e2m1" or "e4m3")."""
     if fmt not in FMT_CODE:
         raise ValueError(f"mx_quantize: fmt is 'e2m1' or 'e4m3', not {fmt!r}")
-    if x.dtype not in DTYPE_CODE or x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError("mx_quantize expects bfloat16, float16 or float32 with a last axis of at least one value")
+    if x.dtype not in DTYPE_CODE or x.dim() < 1 or not 0 < x.shape[-1] <= MAX_WIDTH:
+        raise ValueError("mx_quantize expects bfloat16, float16 or float32 with a last axis of 1 to 2^30 values")
     _ext.refuse_grad("mx_quantize", x)
     if _ext.backend_for(x) != "hip":
         return quantize_reference(x, fmt)

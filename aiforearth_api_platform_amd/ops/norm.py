@@ -153,8 +153,8 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
     strided), ``gamma`` [C] (kept in float32 by a caller that wants no cast per call). Returns the MxTensor and ``h`` in
     x's type, for the next residual (None without ``residual``); the norm is taken of the sum before that rounding."""
     c = x.shape[-1] if x.dim() else 0
-    if x.dtype not in mx.DTYPE_CODE or c == 0:
-        raise ValueError("rms_norm_mx8 expects bfloat16, float16 or float32 with a last axis of at least one value")
+    if x.dtype not in mx.DTYPE_CODE or not 0 < c <= mx.MAX_WIDTH:
+        raise ValueError("rms_norm_mx8 expects bfloat16, float16 or float32 with a last axis of 1 to 2^30 values")
     shape, index = x.shape, x.get_device()
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("rms_norm_mx8: residual has to have x's shape and type")

@@ -74,8 +74,8 @@ struct TileRow {
 
 // The tile kernel: BX x BW outputs per workgroup, WX x WW waves of TX x TW fragments of 32 x 32. Steps of 128 along k go
 // through a ring of STAGES stages in LDS, written by DMA STAGES - 1 steps ahead; a barrier per step. Fragments are read half a
-// step before the matrix instructions that take them.
-template <int FX, int DT, int WX, int WW, int TX, int TW, int STAGES>
+// step before the matrix instructions that take them. SHORT: for fewer than 4 steps, m and n at least 4.
+template <int FX, int DT, int WX, int WW, int TX, int TW, int STAGES, bool SHORT>
 __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w,
     const uint8_t* __restrict__ ws, const float* __restrict__ bias, int m, int n, int kp, int tiles_x, int tiles_w,
@@ -120,11 +120,15 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   for (int j = 0; j < S_DMA; ++j) {
     const int p = (wave + j * NW) % S_ALL;
     soff[j] = static_cast<uint32_t>(p < SX / 64 ? min(p * 64 + lane, m - 1 - x0) : min(p * 64 - SX + lane, n - 1 - w0)) * ps;
+    if (SHORT) {  // the 16 B from a row on pass its end; those of the last rows end with the tensor
+      const int back = p < SX / 64 ? (x0 ? 16 : 0) : (w0 ? 16 : 0);
+      soff[j] = back + min(static_cast<int>(soff[j]), min(p < SX / 64 ? m - x0 : n - w0, 1024) * ps - 16);
+    }
   }
   const uint8_t* xb = x + static_cast<long>(x0) * px;
   const uint8_t* wb = w + static_cast<long>(w0) * pw;
-  const uint8_t* xsb = xs + static_cast<long>(x0) * ps;
-  const uint8_t* wsb = ws + static_cast<long>(w0) * ps;
+  const uint8_t* xsb = xs + static_cast<long>(x0) * ps - (SHORT && x0 ? 16 : 0);
+  const uint8_t* wsb = ws + static_cast<long>(w0) * ps - (SHORT && w0 ? 16 : 0);
 
   const int nk = kp / MX_ALIGN;
   // Where nobody else reads the same rows of w, each workgroup starts elsewhere along k: rows a power of two apart would
@@ -139,7 +143,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 #pragma unroll
     for (int j = 0; j < S_DMA; ++j) {
       const int p = (wave + j * NW) % S_ALL;
-      dma16((p < SX / 64 ? xsb : wsb) + static_cast<long>(place(min(4 * g, nk - 4))) * 4, soff[j],
+      dma16((p < SX / 64 ? xsb : wsb) + (SHORT ? 0 : static_cast<long>(place(min(4 * g, nk - 4))) * 4), soff[j],
             lds0 + SCALES + (g & 1) * S_BYTES + p * 1024);
     }
   };
@@ -182,12 +186,16 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     }
   };
   // a row's four scale bytes of step kt, shifted so that bytes 0 and 2 are those of this half's blocks
+  auto late = [&](int row, int rows) {  // how much earlier than its row a piece of scales begins
+    return SHORT ? max(0, 16 - (min(rows, 1024) - min(row, rows - 1)) * ps) : 0;
+  };
   auto read_scales = [&](int kt, int(&ax)[TX], int(&aw)[TW]) {
-    const uint32_t st = lds0 + SCALES + ((kt >> 2) & 1) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4 + sa;
+    const uint32_t st = lds0 + SCALES + (SHORT ? kt * 4 : ((kt >> 2) & 1) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4) + sa;
 #pragma unroll
-    for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<Lds4>(st + wx * TX * 512 + i * 512);
+    for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<Lds4>(st + wx * TX * 512 + i * 512 + late(xrow + i * 32, m - x0));
 #pragma unroll
-    for (int j = 0; j < TW; ++j) aw[j] = *reinterpret_cast<Lds4>(st + SX * 16 + ww * TW * 512 + j * 512);
+    for (int j = 0; j < TW; ++j)
+      aw[j] = *reinterpret_cast<Lds4>(st + SX * 16 + ww * TW * 512 + j * 512 + late(wrow + j * 32, n - w0));
   };
   auto shift_scales = [&]() {
 #pragma unroll
@@ -231,7 +239,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     __builtin_amdgcn_s_barrier();
     const uint32_t free = slot;
     slot = slot + 1 == STAGES ? 0 : slot + 1;
-    if (((kt + STAGES) & 3) == 0) scales((kt + STAGES) / 4);
+    if (!SHORT && ((kt + STAGES) & 3) == 0) scales((kt + STAGES) / 4);
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       MX_MMA(1, q)
@@ -294,14 +302,14 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   }
 }
 
-template <int FX, int DT, int WX, int WW, int TX, int TW, int STAGES>
+template <int FX, int DT, int WX, int WW, int TX, int TW, int STAGES, bool SHORT = false>
 int launch_tile(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
                 hipStream_t s) {
   constexpr int BX = WX * TX * 32, BW = WW * TW * 32;
   constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES) +
                       2 * ((BX + 63) / 64 * 64 + BW) * 16;
   const int tx = ai4e_cdiv(m, BX), tw = ai4e_cdiv(n, BW);
-  auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES>;
+  auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES, SHORT>;
   static std::atomic<uint64_t> devices{0};
   if (!allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices)) return AI4E_ELAUNCH;
   hipLaunchKernelGGL(kernel, dim3(tx * tw), dim3(WX * WW * 64), LDS, s, static_cast<const uint8_t*>(x),
@@ -395,6 +403,7 @@ template <int FX, int DT, int MT, int NT>
 int launch_slice(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
                  hipStream_t s) {
   const int tm = ai4e_cdiv(m, 16 * MT);
+  if (static_cast<long>(tm) * ai4e_cdiv(n, 16 * NT) >= 1L << 23) return AI4E_EINVAL;  // a launch has fewer than 2^32 threads
   hipLaunchKernelGGL((mx_slice_kernel<FX, DT, MT, NT>), dim3(tm * ai4e_cdiv(n, 16 * NT)), dim3(SLICES * 64), 0, s,
                      static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w),
                      static_cast<const uint8_t*>(ws), static_cast<const float*>(bias), m, n, kp, tm,
@@ -564,14 +573,20 @@ int launch_stream(const void* x, const void* xs, const void* w, const void* ws, 
 //   32 x 128 / stream 2     16 x 24576 x 4096 (192 / 384) 15.7 / 18.3           16 x 16384 x 4096 (128 / 256) 14.2 / 11.0
 //   stream 2 / stream 1     64 x 6144 x 4096 (192 / 384) 9.6 / 11.4             64 x 4096 x 4096 (128 / 256) 7.3 / 6.1
 //   stream 1 / slices       1 x 4096 x 4096 5.6 / 4.4                           16 x 4096 x 4096 5.7 / 5.9
+// and with k below 512, where latency counts more than bytes do:
+//   128 x 128 / 64 x 64     4096 x 16384 x 384 (4096 / 16384 tiles) 52 / 65     1024 x 4096 x 384 (256 / 1024) 7.1 / 6.2
+//   64 x 64 / slices        64 x 16384 x 384 (256 / 512) 3.9 / 5.7              4096 x 16384 x 384 65 / 286
 template <int FX, int DT>
 int launch(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
            hipStream_t s) {
 #define ARGS x, xs, w, ws, bias, m, n, kp, y, s
   const auto blocks = [&](int bm, int bn) { return static_cast<long>(ai4e_cdiv(m, bm)) * ai4e_cdiv(n, bn); };
   constexpr long FILL = 192, ROUND = 320;
-  if (kp < 512)  // the others' scales come four steps of 128 at a time
+  if (kp < 512) {  // the others' scales come four steps of 128 at a time
+    if (m > 64 && n >= 4 && blocks(128, 128) >= 4 * 256) return launch_tile<FX, DT, 2, 2, 2, 2, 2, true>(ARGS);
+    if (m > 32 && n >= 4 && blocks(64, 64) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 1, 2, true>(ARGS);
     return blocks(16, 16) <= ROUND ? launch_slice<FX, DT, 1, 1>(ARGS) : launch_slice<FX, DT, 2, 4>(ARGS);
+  }
   if (m <= 8 && blocks(16, 16) <= ROUND) return launch_slice<FX, DT, 1, 1>(ARGS);
   if (m > 128 && blocks(256, 256) >= FILL) return launch_tile<FX, DT, 4, 2, 2, 4, FX == MX_E4M3 ? 3 : 4>(ARGS);
   if (m > 64 && blocks(128, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 2, 2, FX == MX_E4M3 ? 3 : 4>(ARGS);

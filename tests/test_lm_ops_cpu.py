@@ -172,3 +172,16 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.ai4e_rms_norm_mx8(p, 4, p, 3, p, 1e-6, 1, 4, 0, p, p, p, None) == 1
     assert lib.ai4e_label_logprobs(p, 8, 1, 8, 0, p, 1, 1, 9, p, p, p, p, None) == 1   # k over the classes
     assert lib.ai4e_label_logprobs(p, 8, 1, 8, 0, None, 1, 1, 0, p, p, None, None, None) == 1
+
+
+def test_refusals_of_other_tensors_and_of_rows_past_the_limit():
+    x = mx_quantize(torch.ones(2, 64))
+    for call in (lambda: mx_dequantize(torch.ones(3)), lambda: mx_linear(torch.ones(3, 64), x), lambda: mx_linear(x, x.data)):
+        with pytest.raises(TypeError):
+            call()
+    wide = torch.zeros(1).expand((1 << 30) + 1)  # no memory behind it
+    codes = MxTensor(torch.zeros(1, dtype=torch.uint8).expand(1 << 29), torch.zeros(1, dtype=torch.uint8).expand(1 << 25), 1 << 32)
+    for call in (lambda: mx_quantize(wide), lambda: label_logprobs(wide), lambda: rms_norm_mx8(wide, wide),
+                 lambda: mx_dequantize(codes)):
+        with pytest.raises(ValueError):
+            call()

@@ -164,6 +164,15 @@ def test_linear_scales_at_the_ends_of_their_range():
     assert y.cpu().eq(math.inf).all()
 
 
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", torch.bfloat16), ("e2m1", torch.float32)])
+@pytest.mark.parametrize("m,n,k", [(1793, 1700, 384), (1700, 1793, 200), (2000, 1650, 100), (833, 1030, 384), (40, 12300, 7),
+                                   (12289, 4, 300), (24577, 5, 128), (30000, 3, 128), (33, 12289, 256),
+                                   (4097, 4100, 130), (131073, 4, 384)])
+def test_linear_short_rows(m, n, k, fmt, dtype):
+    """Fewer than 4 steps of k: tiles whose last rows' scales end with the tensor, and the slices where no tile fits."""
+    check_linear(m, n, k, fmt, dtype, bias=True, seed=m)
+
+
 def test_linear_same_call_same_bits():
     g = gen(9)
     for m, n, k in ((1, 512, 4096), (16, 1024, 8192), (200, 300, 4096)):
