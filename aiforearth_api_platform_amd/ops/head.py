@@ -64,10 +64,10 @@ def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, 
     if _ext.backend_for(logits) != "hip":
         return _label_logprobs_reference(logits, labels, n_labels, k)
     dev = logits.device
-    logp = None if labels is None else torch.empty(labels.shape, device=dev, dtype=torch.float32)
-    entropy = torch.empty(lead, device=dev, dtype=torch.float32)
-    top_idx = torch.empty((*lead, k), device=dev, dtype=torch.int32)
-    top_logp = torch.empty((*lead, k), device=dev, dtype=torch.float32)
+    logp = None if labels is None else mx.new(labels.shape, torch.float32, dev)
+    entropy = mx.new(lead, torch.float32, dev)
+    top_idx = mx.new((*lead, k), torch.int32, dev)
+    top_logp = mx.new((*lead, k), torch.float32, dev)
     x = mx.rows_2d(logits)
     rows = x.shape[0]
     if rows:

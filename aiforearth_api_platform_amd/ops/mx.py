@@ -54,12 +54,20 @@ def padded(k: int) -> int:
     return -(-k // ALIGN) * ALIGN
 
 
+def new(shape, dtype: torch.dtype, device) -> torch.Tensor:
+    """An uninitialised contiguous tensor (of few axes by its strides, 0.5 us less than ``torch.empty`` takes)."""
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1], 1), dtype=dtype, device=device)
+    if len(shape) == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
 def empty(lead, k: int, fmt: str, device) -> MxTensor:
     """An uninitialised MxTensor of ``(*lead, k)``."""
     kp = padded(k)
-    data = (torch.empty((*lead, kp), device=device, dtype=torch.float8_e4m3fn) if fmt == "e4m3"
-            else torch.empty((*lead, kp // 2), device=device, dtype=torch.uint8))
-    return MxTensor(data, torch.empty((*lead, kp // BLOCK), device=device, dtype=torch.float8_e8m0fnu), k)
+    data = new((*lead, kp), torch.float8_e4m3fn, device) if fmt == "e4m3" else new((*lead, kp // 2), torch.uint8, device)
+    return MxTensor(data, new((*lead, kp // BLOCK), torch.float8_e8m0fnu, device), k)
 
 
 def check(name: str, q: MxTensor) -> None:
@@ -146,7 +154,7 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
         raise ValueError("mx_dequantize gives bfloat16, float16 or float32")
     if _ext.backend_for(q.data) != "hip":
         return dequantize_reference(q).to(dtype)
-    y = torch.empty(q.shape, device=q.device, dtype=dtype)
+    y = new(q.shape, dtype, q.data.device)
     if y.numel():
         _ext.call_on(y.get_device(), "ai4e_mx_dequantize", q.data.data_ptr(), q.scale.data_ptr(), y.numel() // q.k, q.k,
                      DTYPE_CODE[dtype], FMT_CODE[q.fmt], y.data_ptr())
@@ -183,7 +191,7 @@ def mx_linear(x: MxTensor, w: MxTensor, bias: Optional[torch.Tensor] = None,
     if _ext.backend_for(data) != "hip":
         y = dequantize_reference(x) @ dequantize_reference(w).T
         return (y if bias is None else y + bias.float()).to(out_dtype)
-    y = torch.empty((*data.shape[:-1], n), device=data.device, dtype=out_dtype)
+    y = new((*data.shape[:-1], n), out_dtype, data.device)
     if y.numel():
         b32 = None if bias is None else bias.to(torch.float32).contiguous()
         _ext.call_on(index, "ai4e_mx_linear", data.data_ptr(), scale.data_ptr(), FMT_CODE[fmt], w.data.data_ptr(),

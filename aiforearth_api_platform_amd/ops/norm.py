@@ -170,7 +170,7 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
         y = h.double() / torch.sqrt(h.double().square().mean(-1, keepdim=True) + eps) * gamma.double()
         return mx.quantize_reference(y.float(), "e4m3"), None if residual is None else h.to(x.dtype)
     q = mx.empty(shape[:-1], c, "e4m3", x.device)
-    h = None if residual is None else torch.empty(shape, device=x.device, dtype=x.dtype)
+    h = None if residual is None else mx.new(shape, x.dtype, x.device)
     g32 = gamma if gamma.dtype == torch.float32 and gamma.is_contiguous() else gamma.to(torch.float32).contiguous()
     x2 = mx.rows_2d(x)
     r2 = None if residual is None else mx.rows_2d(residual)
