@@ -167,7 +167,8 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
     _ext.refuse_grad("rms_norm_mx8", x, gamma, residual)
     if _ext.backend_for(x) != "hip":
         h = x.float() if residual is None else x.float() + residual.float()
-        y = h.double() / torch.sqrt(h.double().square().mean(-1, keepdim=True) + eps) * gamma.double()
+        h64 = h.double() if residual is None else torch.where(h.isfinite(), x.double() + residual.double(), h.double())
+        y = h64 / torch.sqrt(h64.square().mean(-1, keepdim=True) + eps) * gamma.double()
         return mx.quantize_reference(y.float(), "e4m3"), None if residual is None else h.to(x.dtype)
     q = mx.empty(shape[:-1], c, "e4m3", x.device)
     h = None if residual is None else mx.new(shape, x.dtype, x.device)

@@ -238,6 +238,28 @@ def test_rms_norm_ranges_and_not_finite(c):
     check_norm(x.bfloat16(), torch.rand(c, generator=g) + 0.5, torch.zeros(9, c).bfloat16())
 
 
+@pytest.mark.parametrize("dtype,c,with_residual", [(torch.float32, 2500, True), (torch.float32, 700, False),
+                                                   (torch.bfloat16, 4096, True), (torch.float16, 20000, True)])
+def test_rms_norm_elements_are_the_exact_values_neighbours(dtype, c, with_residual):
+    """y is held to some 2^-40 of itself: of a million elements, whose borders are 2^-4 apart, none falls to the other side."""
+    g = gen(c)
+    x = torch.randn(1 << 20, generator=g)[:(1 << 20) // c * c].view(-1, c).to(dtype)
+    r = torch.randn(x.shape, generator=g).to(dtype) if with_residual else None
+    gamma = torch.rand(c, generator=g) + 0.5
+    q, _ = rms_norm_mx8(x.to(DEV), gamma.to(DEV), None if r is None else r.to(DEV))
+    assert torch.equal(mx_dequantize(q).cpu().double(), oracle.mx_values(oracle.rms_norm(x, gamma, r, 1e-6), "e4m3"))
+
+
+def test_rms_norm_sum_past_the_type():
+    """A 32-bit sum that overflows is an infinity: its block is not finite, what else is in the row becomes 0."""
+    x = torch.ones(2, 96)
+    x[0, 40] = 3e38
+    for dev in ("cpu", DEV):
+        q, h = rms_norm_mx8(x.to(dev), torch.ones(96, device=dev), x.to(dev))
+        assert q.scale.view(torch.uint8).cpu()[0].tolist() == [0, 255, 0, 0] and math.isinf(h[0, 40].item())
+        assert q.data.view(torch.uint8)[0].eq(0).all() and torch.equal(mx_dequantize(q)[1].cpu(), torch.ones(96))
+
+
 def test_rms_norm_strided_and_leading_axes():
     g = gen(4)
     x, r = torch.randn(6, 5, 333, generator=g).half(), torch.randn(6, 5, 333, generator=g).half()
