@@ -91,7 +91,8 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   constexpr int X_DMA = (X_ALL + NW - 1) / NW, W_DMA = (W_ALL + NW - 1) / NW, S_DMA = (S_ALL + NW - 1) / NW;
   constexpr int PER_STAGE = X_DMA + W_DMA;
   static_assert(X_BYTES % 1024 == 0 && W_BYTES % 1024 == 0 && S_BYTES % 1024 == 0, "");
-  static_assert(SCALES + 2 * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 4, "");
+  constexpr int SLOTS = STAGES > 4 ? 4 : 2;  // of the scales of 4 steps
+  static_assert(SCALES + SLOTS * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 8, "");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -138,13 +139,13 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
       (__attribute__((address_space(3))) uint8_t*)lds));
   // scales come 16 B of a row at a time, for 4 steps: as 4-B pieces they would be as many requests to L2 as the data
-  // (measured: the rate of requests was what bound the kernel). Two slots; the last group ends with the row.
+  // (measured: the rate of requests was what bound the kernel). The last group ends with the row.
   auto scales = [&](int g) {
 #pragma unroll
     for (int j = 0; j < S_DMA; ++j) {
       const int p = (wave + j * NW) % S_ALL;
       dma16((p < SX / 64 ? xsb : wsb) + (SHORT ? 0 : static_cast<long>(place(min(4 * g, nk - 4))) * 4), soff[j],
-            lds0 + SCALES + (g & 1) * S_BYTES + p * 1024);
+            lds0 + SCALES + (g & (SLOTS - 1)) * S_BYTES + p * 1024);
     }
   };
   // piece j of step kt; past the end the last step is brought again, into a slot that nobody reads
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     return SHORT ? max(0, 16 - (min(rows, 1024) - min(row, rows - 1)) * ps) : 0;
   };
   auto read_scales = [&](int kt, int(&ax)[TX], int(&aw)[TW]) {
-    const uint32_t st = lds0 + SCALES + (SHORT ? kt * 4 : ((kt >> 2) & 1) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4) + sa;
+    const uint32_t st = lds0 + SCALES + (SHORT ? kt * 4 : ((kt >> 2) & (SLOTS - 1)) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4) + sa;
 #pragma unroll
     for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<Lds4>(st + wx * TX * 512 + i * 512 + late(xrow + i * 32, m - x0));
 #pragma unroll
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 
 #pragma unroll
   for (int s = 0; s < STAGES; ++s) {
-    if (s == 0) scales(0);
+    if (s % 4 == 0) scales(s / 4);
 #pragma unroll
     for (int j = 0; j < PER_STAGE; ++j) issue(s, s, j);
   }
@@ -307,7 +308,7 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
                 hipStream_t s) {
   constexpr int BX = WX * TX * 32, BW = WW * TW * 32;
   constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES) +
-                      2 * ((BX + 63) / 64 * 64 + BW) * 16;
+                      (STAGES > 4 ? 4 : 2) * ((BX + 63) / 64 * 64 + BW) * 16;
   const int tx = ai4e_cdiv(m, BX), tw = ai4e_cdiv(n, BW);
   auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES, SHORT>;
   static std::atomic<uint64_t> devices{0};
@@ -594,7 +595,7 @@ int launch(const void* x, const void* xs, const void* w, const void* ws, const v
   if (m > 32 && blocks(64, 64) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
   if (blocks(32, 32) <= ROUND) return launch_stream<FX, DT, 1, 2>(ARGS);
   if (blocks(32, 64) <= ROUND) return launch_stream<FX, DT, 2, 2>(ARGS);
-  return m <= 32 ? launch_tile<FX, DT, 1, 4, 1, 1, 4>(ARGS) : launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
+  return m <= 32 ? launch_tile<FX, DT, 1, 4, 1, 1, 8>(ARGS) : launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
 #undef ARGS
 }
 
