@@ -133,7 +133,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 
   const int nk = kp / MX_ALIGN;
   // Where nobody else reads the same rows of w, each workgroup starts elsewhere along k: rows a power of two apart would
-  // else have all workgroups in the same memory channels at once (16 x 32768 x 8192 35 us, so 31). Whole groups of scales.
+  // else have all workgroups in the same memory channels at once (16 x 32768 x 16384 50 us, so 46). Whole groups of scales.
   const int rot = tiles_x > 1 || nk % 4 ? 0 : w0 / BW * 5 * 4 % nk;
   auto place = [&](int k) { return k + rot < nk ? k + rot : k + rot - nk; };
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
@@ -571,7 +571,7 @@ int launch_stream(const void* x, const void* xs, const void* w, const void* ws, 
 //   128 x 128 / 64 x 128    512 x 4096 x 4096 (128 / 256 tiles) 17.6 / 12.5     512 x 8192 x 8192 (256 / 512) 38.5 / 45.0
 //   64 x 128 / 64 x 64      256 x 4096 x 4096 (128 / 256 tiles) 12.5 / 10.9     256 x 8192 x 8192 (256 / 512) 26.4 / 33.0
 //   64 x 64 / stream 2      128 x 4096 x 4096 (128 / 256) 10.6 / 7.8            200 x 3000 x 4096 (188 / 329) 11.0 / 11.4
-//   32 x 128 / stream 2     16 x 24576 x 4096 (192 / 384) 15.7 / 18.3           16 x 16384 x 4096 (128 / 256) 14.2 / 11.0
+//   32 x 128 / stream 2     16 x 20480 x 4096 (160 / 320) 11.9 / 13.5           16 x 16384 x 4096 (128 / 256) 11.6 / 9.7
 //   stream 2 / stream 1     64 x 6144 x 4096 (192 / 384) 9.6 / 11.4             64 x 4096 x 4096 (128 / 256) 7.3 / 6.1
 //   stream 1 / slices       1 x 4096 x 4096 5.6 / 4.4                           16 x 4096 x 4096 5.7 / 5.9
 // and with k below 512, where latency counts more than bytes do:
@@ -594,7 +594,7 @@ int launch(const void* x, const void* xs, const void* w, const void* ws, const v
   if (m > 32 && blocks(64, 128) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 2, 4>(ARGS);
   if (m > 32 && blocks(64, 64) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
   if (blocks(32, 32) <= ROUND) return launch_stream<FX, DT, 1, 2>(ARGS);
-  if (blocks(32, 64) <= ROUND) return launch_stream<FX, DT, 2, 2>(ARGS);
+  if (blocks(32, 64) <= (m > 32 ? ROUND : 256)) return launch_stream<FX, DT, 2, 2>(ARGS);
   return m <= 32 ? launch_tile<FX, DT, 1, 4, 1, 1, 8>(ARGS) : launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
 #undef ARGS
 }
