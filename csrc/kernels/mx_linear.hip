@@ -91,8 +91,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   constexpr int X_DMA = (X_ALL + NW - 1) / NW, W_DMA = (W_ALL + NW - 1) / NW, S_DMA = (S_ALL + NW - 1) / NW;
   constexpr int PER_STAGE = X_DMA + W_DMA;
   static_assert(X_BYTES % 1024 == 0 && W_BYTES % 1024 == 0 && S_BYTES % 1024 == 0, "");
-  constexpr int SLOTS = STAGES > 4 ? 4 : 2;  // of the scales of 4 steps
-  static_assert(SCALES + SLOTS * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 8, "");
+  static_assert(SCALES + 2 * S_BYTES <= 160 * 1024 && STAGES >= 2 && STAGES <= 4, "");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -133,19 +132,19 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 
   const int nk = kp / MX_ALIGN;
   // Where nobody else reads the same rows of w, each workgroup starts elsewhere along k: rows a power of two apart would
-  // else have all workgroups in the same memory channels at once (16 x 32768 x 16384 50 us, so 46). Whole groups of scales.
+  // else have all workgroups in the same memory channels at once (16 x 32768 x 8192 36 us, so 32). Whole groups of scales.
   const int rot = tiles_x > 1 || nk % 4 ? 0 : w0 / BW * 5 * 4 % nk;
   auto place = [&](int k) { return k + rot < nk ? k + rot : k + rot - nk; };
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
       (__attribute__((address_space(3))) uint8_t*)lds));
   // scales come 16 B of a row at a time, for 4 steps: as 4-B pieces they would be as many requests to L2 as the data
-  // (measured: the rate of requests was what bound the kernel). The last group ends with the row.
+  // (measured: the rate of requests was what bound the kernel). Two slots; the last group ends with the row.
   auto scales = [&](int g) {
 #pragma unroll
     for (int j = 0; j < S_DMA; ++j) {
       const int p = (wave + j * NW) % S_ALL;
       dma16((p < SX / 64 ? xsb : wsb) + (SHORT ? 0 : static_cast<long>(place(min(4 * g, nk - 4))) * 4), soff[j],
-            lds0 + SCALES + (g & (SLOTS - 1)) * S_BYTES + p * 1024);
+            lds0 + SCALES + (g & 1) * S_BYTES + p * 1024);
     }
   };
   // piece j of step kt; past the end the last step is brought again, into a slot that nobody reads
@@ -191,7 +190,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     return SHORT ? max(0, 16 - (min(rows, 1024) - min(row, rows - 1)) * ps) : 0;
   };
   auto read_scales = [&](int kt, int(&ax)[TX], int(&aw)[TW]) {
-    const uint32_t st = lds0 + SCALES + (SHORT ? kt * 4 : ((kt >> 2) & (SLOTS - 1)) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4) + sa;
+    const uint32_t st = lds0 + SCALES + (SHORT ? kt * 4 : ((kt >> 2) & 1) * S_BYTES + (kt - min(kt & ~3, nk - 4)) * 4) + sa;
 #pragma unroll
     for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<Lds4>(st + wx * TX * 512 + i * 512 + late(xrow + i * 32, m - x0));
 #pragma unroll
@@ -213,7 +212,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 
 #pragma unroll
   for (int s = 0; s < STAGES; ++s) {
-    if (s % 4 == 0) scales(s / 4);
+    if (s == 0) scales(0);
 #pragma unroll
     for (int j = 0; j < PER_STAGE; ++j) issue(s, s, j);
   }
@@ -308,7 +307,7 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
                 hipStream_t s) {
   constexpr int BX = WX * TX * 32, BW = WW * TW * 32;
   constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES) +
-                      (STAGES > 4 ? 4 : 2) * ((BX + 63) / 64 * 64 + BW) * 16;
+                      2 * ((BX + 63) / 64 * 64 + BW) * 16;
   const int tx = ai4e_cdiv(m, BX), tw = ai4e_cdiv(n, BW);
   auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES, SHORT>;
   static std::atomic<uint64_t> devices{0};
@@ -566,12 +565,13 @@ int launch_stream(const void* x, const void* xs, const void* w, const void* ws, 
 
 // Which kernel: the largest tile that still gives most of the 256 CUs one, since a larger tile moves fewer bytes per
 // product; where even 64 x 64 does not, the streams that need one round of workgroups, and for the fewest rows slices.
-// Measured at the borders (us, e4m3, cold weights; the first kernel's time first):
+// Measured at the borders (us, e4m3; the first kernel's time first; weights from memory where a row names 16 rows of x,
+// else from the memory-side cache):
 //   256 x 256 / 128 x 128   1024 x 8192 x 8192 (128 / 512 tiles) 77.7 / 61.8    4096 x 4096 x 4096 (256 / 1024) 55 / 70
 //   128 x 128 / 64 x 128    512 x 4096 x 4096 (128 / 256 tiles) 17.6 / 12.5     512 x 8192 x 8192 (256 / 512) 38.5 / 45.0
 //   64 x 128 / 64 x 64      256 x 4096 x 4096 (128 / 256 tiles) 12.5 / 10.9     256 x 8192 x 8192 (256 / 512) 26.4 / 33.0
 //   64 x 64 / stream 2      128 x 4096 x 4096 (128 / 256) 10.6 / 7.8            200 x 3000 x 4096 (188 / 329) 11.0 / 11.4
-//   32 x 128 / stream 2     16 x 20480 x 4096 (160 / 320) 11.9 / 13.5           16 x 16384 x 4096 (128 / 256) 11.6 / 9.7
+//   32 x 128 / stream 2     16 x 20480 x 4096 (160 / 320) 15.2 / 17.9           16 x 16384 x 4096 (128 / 256) 13.6 / 10.9
 //   stream 2 / stream 1     64 x 6144 x 4096 (192 / 384) 9.6 / 11.4             64 x 4096 x 4096 (128 / 256) 7.3 / 6.1
 //   stream 1 / slices       1 x 4096 x 4096 5.6 / 4.4                           16 x 4096 x 4096 5.7 / 5.9
 // and with k below 512, where latency counts more than bytes do:
@@ -595,7 +595,7 @@ int launch(const void* x, const void* xs, const void* w, const void* ws, const v
   if (m > 32 && blocks(64, 64) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
   if (blocks(32, 32) <= ROUND) return launch_stream<FX, DT, 1, 2>(ARGS);
   if (blocks(32, 64) <= (m > 32 ? ROUND : 256)) return launch_stream<FX, DT, 2, 2>(ARGS);
-  return m <= 32 ? launch_tile<FX, DT, 1, 4, 1, 1, 8>(ARGS) : launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
+  return m <= 32 ? launch_tile<FX, DT, 1, 4, 1, 1, 4>(ARGS) : launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
 #undef ARGS
 }
 
