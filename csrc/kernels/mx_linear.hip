@@ -22,18 +22,30 @@ typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef i32x4_t __attribute__((aligned(2))) Chunk16;  // 16 B of outputs: rows of odd n start at any element
 
 // 16 B per lane from base + off to LDS at (wave-uniform lds + 16 * lane); completion is counted by vmcnt.
-// M0 is put back: the compiler reserves it.
+// M0 is put back: the compiler reserves it. PAST: past the caches, for what is read once.
+template <bool PAST = false>
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds) {
   uint32_t keep;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %2\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(keep)
-      : "v"(off), "s"(base), "s"(lds)
-      : "memory");
+  if constexpr (PAST)
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2 nt\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "v"(off), "s"(base), "s"(lds)
+        : "memory");
+  else
+    asm volatile(
+        "s_mov_b32 %0, m0\n\t"
+        "s_mov_b32 m0, %3\n\t"
+        "s_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, %2\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "v"(off), "s"(base), "s"(lds)
+        : "memory");
 }
 
 // Dynamic LDS over 64 KB is allowed per kernel and device, before its first launch there. `devices`: where it is.
@@ -318,6 +330,154 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
   return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
 }
 
+// The few-rows kernel: up to 32 rows of x by 128 rows of w per workgroup of 4 waves, a fragment of 32 x 32 each. What
+// bounds it is how w comes out of memory: a DMA brings 256 consecutive bytes of 4 rows, four steps of k, since pieces of one
+// step (64 B) of many rows take longer (16 x 32768 x 8192 31.5 us, so 30.2), and past the caches, since a model's weights come by
+// once per token (26.9; weights that a cache still holds 25.5 us, through it 24.0). Such groups of four steps go through a
+// ring of three, two of them in flight, a barrier per group, from one tile of a workgroup to its next.
+template <int FX, int DT>
+struct FewLds {
+  static constexpr int X_ROW = 4 * TileRow<FX>::BYTES, W_ROW = 4 * TileRow<MX_E2M1>::BYTES;  // bytes of a row of a group
+  static constexpr int X_BYTES = 32 * X_ROW, W_BYTES = 128 * W_ROW, S_BYTES = (64 + 128) * 16;
+  static constexpr int GROUP = X_BYTES + W_BYTES + S_BYTES, RING = 3, ALL = RING * GROUP;
+  static_assert(ALL <= 160 * 1024, "");
+};
+
+template <int FX, int DT>
+__global__ __launch_bounds__(256) void mx_few_kernel(
+    const uint8_t* __restrict__ x, const uint8_t* __restrict__ xs, const uint8_t* __restrict__ w,
+    const uint8_t* __restrict__ ws, const float* __restrict__ bias, int m, int n, int kp, int tiles,
+    typename mx_elem<DT>::type* __restrict__ y) {
+  typedef FewLds<FX, DT> S;
+  constexpr int X_DMA = S::X_BYTES / 1024 / 4, W_DMA = S::W_BYTES / 1024 / 4, PER_GROUP = X_DMA + W_DMA + 1;
+  constexpr int X_CHUNKS = S::X_ROW / 16, W_CHUNKS = S::W_ROW / 16;  // of 16 B; stored at their place ^ (row & 15)
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, half = lane >> 5, r = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int px = FX == MX_E4M3 ? kp : kp / 2, pw = kp / 2, ps = kp / 32;
+  uint32_t xoff[X_DMA], woff[W_DMA];
+#pragma unroll
+  for (int j = 0; j < X_DMA; ++j) {
+    const int row = ((wave * X_DMA + j) * 64 + lane) / X_CHUNKS;
+    xoff[j] = static_cast<uint32_t>(min(row, m - 1)) * px + ((lane % X_CHUNKS) ^ (row & 15)) * 16;
+  }
+#pragma unroll
+  for (int j = 0; j < W_DMA; ++j) {
+    const int row = ((wave * W_DMA + j) * 64 + lane) / W_CHUNKS;
+    woff[j] = static_cast<uint32_t>(row) * pw + ((lane % W_CHUNKS) ^ (row & 15)) * 16;
+  }
+  // scales of 64 rows per DMA: w's two halves, x's rows, and those once more
+  const uint32_t soff = static_cast<uint32_t>(wave < 2 ? wave * 64 + lane : min(lane, m - 1)) * ps;
+  const uint32_t sto = S::X_BYTES + S::W_BYTES + (wave < 2 ? wave : 2) * 1024;
+
+  // the workgroup's tiles one after the other, all the groups of each; a workgroup's first group lies elsewhere along k
+  // than its neighbours', since rows a power of two apart would else be in the same memory channels at once
+  const int nk = kp / MX_ALIGN, groups = (nk + 3) / 4;
+  const int mine = (tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  struct Place {
+    int tile, group;
+  };
+  const int rot = blockIdx.x * 5 % groups;
+  Place next = {0, 0}, now = {0, 0};  // the group to fetch, the group at work: tile of this workgroup, turn in the tile
+  auto advance = [&](Place& p) {
+    if (++p.group == groups) {
+      p.group = 0;
+      ++p.tile;
+    }
+  };
+  auto place = [&](const Place& p) { return p.group + rot < groups ? p.group + rot : p.group + rot - groups; };
+  // a tile's first row of w: n is at least 128, and the last tile ends with w
+  auto start = [&](int t) { return min(static_cast<int>(blockIdx.x + t * gridDim.x) * 128, n - 128); };
+  const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) uint8_t*)lds));
+  auto issue = [&](uint32_t slot) {  // past the end the last tile's groups are brought again, into slots that nobody reads
+    const int k = __builtin_amdgcn_readfirstlane(min(4 * place(next), nk - 4));  // the last group ends with the row
+    const int w0 = start(min(next.tile, mine - 1));
+    advance(next);
+    const uint32_t base = lds0 + slot * S::GROUP;
+    dma16((wave < 2 ? ws + static_cast<long>(w0) * ps : xs) + k * 4l, soff, base + sto);
+    const uint8_t* wb = w + static_cast<long>(w0) * pw + k * 64l;
+#pragma unroll
+    for (int j = 0; j < W_DMA; ++j) dma16<true>(wb, woff[j], base + S::X_BYTES + (wave * W_DMA + j) * 1024);
+#pragma unroll
+    for (int j = 0; j < X_DMA; ++j)
+      dma16(x + k * static_cast<long>(TileRow<FX>::BYTES), xoff[j], base + (wave * X_DMA + j) * 1024);
+  };
+  typedef __attribute__((address_space(3))) const i32x4_t* Lds16;
+  typedef __attribute__((address_space(3))) const int* Lds4;
+  const uint32_t xa = r * S::X_ROW, wa = S::X_BYTES + (wave * 32 + r) * S::W_ROW;
+  const uint32_t sa = S::X_BYTES + S::W_BYTES + (wave * 32 + r) * 16;
+  f32x16_t acc = {};
+  issue(0);
+  issue(1);
+  uint32_t slot = 0;
+  while (now.tile < mine) {
+    // this wave's part of the group is there and it has read all of the last one: after the barrier the group is complete
+    // and the last one's slot free
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(PER_GROUP) : "memory");
+    __builtin_amdgcn_s_barrier();
+    issue(slot == 0 ? 2 : slot - 1);
+    const uint32_t st = lds0 + slot * S::GROUP;
+    const int p0 = max(0, 4 * place(now) - (nk - 4));  // steps that the last group shares with the one before it
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      if (p < p0) continue;
+      const int sw = *reinterpret_cast<Lds4>(st + sa + p * 4) >> (8 * half);
+      const int sx = *reinterpret_cast<Lds4>(st + S::X_BYTES + S::W_BYTES + 2048 + r * 16 + p * 4) >> (8 * half);
+      i32x8_t fx[2], fw[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const i32x4_t a = *reinterpret_cast<Lds16>(st + wa + ((4 * p + 2 * u + half) ^ (r & 15)) * 16);
+        fw[u] = __builtin_shufflevector(a, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
+        if constexpr (FX == MX_E4M3) {
+          const i32x4_t b = *reinterpret_cast<Lds16>(st + xa + ((8 * p + 4 * u + half) ^ (r & 15)) * 16);
+          const i32x4_t c = *reinterpret_cast<Lds16>(st + xa + ((8 * p + 4 * u + 2 + half) ^ (r & 15)) * 16);
+          fx[u] = __builtin_shufflevector(b, c, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+          const i32x4_t b = *reinterpret_cast<Lds16>(st + xa + ((4 * p + 2 * u + half) ^ (r & 15)) * 16);
+          fx[u] = __builtin_shufflevector(b, i32x4_t{}, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+      }
+      acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[0], fx[0], acc, 4, FX == MX_E4M3 ? 0 : 4, 0, sw, 0, sx);
+      acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fw[1], fx[1], acc, 4, FX == MX_E4M3 ? 0 : 4, 2, sw, 2, sx);
+    }
+    slot = slot == 2 ? 0 : slot + 1;
+    if (now.group == groups - 1) {
+      const int w0 = start(now.tile) + wave * 32, from = (blockIdx.x + now.tile * gridDim.x) * 128;
+      if (r < m)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int col = w0 + 8 * q + 4 * half;
+          const f32x4_t v = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+          if (col >= from) {
+            store4<DT>(y + static_cast<long>(r) * n, col, n, bias, v);
+          } else {  // columns below `from` are the tile's before this one
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+              if (col + p >= from) y[static_cast<long>(r) * n + col + p] = mx_elem<DT>::from(v[p] + (bias ? bias[col + p] : 0.f));
+          }
+        }
+      acc = f32x16_t{};
+    }
+    advance(now);
+  }
+  ai4e_conv::wait_vmcnt<0>();  // the ring is the workgroup's until the last DMA has landed
+}
+
+template <int FX, int DT>
+int launch_few(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
+               hipStream_t s) {
+  constexpr int LDS = FewLds<FX, DT>::ALL;
+  auto* kernel = mx_few_kernel<FX, DT>;
+  static std::atomic<uint64_t> devices{0};
+  if (!allow_lds(reinterpret_cast<const void*>(kernel), LDS, devices)) return AI4E_ELAUNCH;
+  const int tiles = ai4e_cdiv(n, 128);
+  hipLaunchKernelGGL(kernel, dim3(tiles < 256 ? tiles : 256), dim3(256), LDS, s, static_cast<const uint8_t*>(x),
+                     static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(ws),
+                     static_cast<const float*>(bias), m, n, kp, tiles, static_cast<typename mx_elem<DT>::type*>(y));
+  return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
+}
+
 // The slice kernel: 16 MT rows of x by 16 NT rows of w per workgroup, k cut over its 8 waves: for the fewest rows, where
 // latency counts, and for k below 512. Operands go from memory to registers, in steps of v_mfma_scale_f32_16x16x128: lane l
 // holds row l & 15, k = 32 (l >> 4) .. + 31 of e2m1, 16 (l >> 4) .. + 15 and 64 + 16 (l >> 4) .. + 15 of e4m3, the scale
@@ -595,7 +755,7 @@ int launch(const void* x, const void* xs, const void* w, const void* ws, const v
   if (m > 32 && blocks(64, 64) >= FILL) return launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
   if (blocks(32, 32) <= ROUND) return launch_stream<FX, DT, 1, 2>(ARGS);
   if (blocks(32, 64) <= (m > 32 ? ROUND : 256)) return launch_stream<FX, DT, 2, 2>(ARGS);
-  return m <= 32 ? launch_tile<FX, DT, 1, 4, 1, 1, 4>(ARGS) : launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
+  return m <= 32 ? launch_few<FX, DT>(ARGS) : launch_tile<FX, DT, 2, 2, 1, 1, 4>(ARGS);
 #undef ARGS
 }
 

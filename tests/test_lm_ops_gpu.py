@@ -173,6 +173,13 @@ def test_linear_short_rows(m, n, k, fmt, dtype):
     check_linear(m, n, k, fmt, dtype, bias=True, seed=m)
 
 
+@pytest.mark.parametrize("fmt,dtype", [("e4m3", torch.bfloat16), ("e2m1", torch.float32)])
+@pytest.mark.parametrize("m,n,k", [(1, 33000, 512), (32, 24600, 2500), (17, 65700, 640), (9, 40001, 1152), (31, 33300, 896)])
+def test_linear_few_rows(m, n, k, fmt, dtype):
+    """Up to 32 rows over several tiles of a workgroup, the last one ragged; a last group of k that shares steps."""
+    check_linear(m, n, k, fmt, dtype, bias=True, seed=n)
+
+
 def test_linear_same_call_same_bits():
     g = gen(9)
     for m, n, k in ((1, 512, 4096), (16, 1024, 8192), (200, 300, 4096)):
