@@ -95,8 +95,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
   constexpr int NW = WX * WW, BX = WX * TX * 32, BW = WW * TW * 32;
   typedef TileRow<FX> XR;
   typedef TileRow<MX_E2M1> WR;
-  constexpr int SX = (BX + 63) / 64 * 64;  // scales of x come for whole sets of 64 rows
-  constexpr int X_BYTES = BX * XR::BYTES, W_BYTES = BW * WR::BYTES, S_BYTES = (SX + BW) * 16;
+  constexpr int X_BYTES = BX * XR::BYTES, W_BYTES = BW * WR::BYTES, S_BYTES = (BX + BW) * 16;
   constexpr int STAGE = X_BYTES + W_BYTES, SCALES = STAGE * STAGES;
   // DMAs per stage; the waves that a tile's DMAs do not divide among bring some twice
   constexpr int X_ALL = X_BYTES / 1024, W_ALL = W_BYTES / 1024, S_ALL = S_BYTES / 1024;
@@ -131,10 +130,10 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 #pragma unroll
   for (int j = 0; j < S_DMA; ++j) {
     const int p = (wave + j * NW) % S_ALL;
-    soff[j] = static_cast<uint32_t>(p < SX / 64 ? min(p * 64 + lane, m - 1 - x0) : min(p * 64 - SX + lane, n - 1 - w0)) * ps;
+    soff[j] = static_cast<uint32_t>(p < BX / 64 ? min(p * 64 + lane, m - 1 - x0) : min(p * 64 - BX + lane, n - 1 - w0)) * ps;
     if (SHORT) {  // the 16 B from a row on pass its end; those of the last rows end with the tensor
-      const int back = p < SX / 64 ? (x0 ? 16 : 0) : (w0 ? 16 : 0);
-      soff[j] = back + min(static_cast<int>(soff[j]), min(p < SX / 64 ? m - x0 : n - w0, 1024) * ps - 16);
+      const int back = p < BX / 64 ? (x0 ? 16 : 0) : (w0 ? 16 : 0);
+      soff[j] = back + min(static_cast<int>(soff[j]), min(p < BX / 64 ? m - x0 : n - w0, 1024) * ps - 16);
     }
   }
   const uint8_t* xb = x + static_cast<long>(x0) * px;
@@ -144,7 +143,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 
   const int nk = kp / MX_ALIGN;
   // Where nobody else reads the same rows of w, each workgroup starts elsewhere along k: rows a power of two apart would
-  // else have all workgroups in the same memory channels at once (16 x 32768 x 8192 36 us, so 32). Whole groups of scales.
+  // else have all workgroups in the same memory channels at once (64 x 32768 x 8192, weights out of memory: 41.0 us, so 38.8). Whole groups of scales.
   const int rot = tiles_x > 1 || nk % 4 ? 0 : w0 / BW * 5 * 4 % nk;
   auto place = [&](int k) { return k + rot < nk ? k + rot : k + rot - nk; };
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
@@ -155,7 +154,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
 #pragma unroll
     for (int j = 0; j < S_DMA; ++j) {
       const int p = (wave + j * NW) % S_ALL;
-      dma16((p < SX / 64 ? xsb : wsb) + (SHORT ? 0 : static_cast<long>(place(min(4 * g, nk - 4))) * 4), soff[j],
+      dma16((p < BX / 64 ? xsb : wsb) + (SHORT ? 0 : static_cast<long>(place(min(4 * g, nk - 4))) * 4), soff[j],
             lds0 + SCALES + (g & 1) * S_BYTES + p * 1024);
     }
   };
@@ -207,7 +206,7 @@ __global__ __launch_bounds__(WX* WW * 64) void mx_tile_kernel(
     for (int i = 0; i < TX; ++i) ax[i] = *reinterpret_cast<Lds4>(st + wx * TX * 512 + i * 512 + late(xrow + i * 32, m - x0));
 #pragma unroll
     for (int j = 0; j < TW; ++j)
-      aw[j] = *reinterpret_cast<Lds4>(st + SX * 16 + ww * TW * 512 + j * 512 + late(wrow + j * 32, n - w0));
+      aw[j] = *reinterpret_cast<Lds4>(st + BX * 16 + ww * TW * 512 + j * 512 + late(wrow + j * 32, n - w0));
   };
   auto shift_scales = [&]() {
 #pragma unroll
@@ -319,7 +318,7 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
                 hipStream_t s) {
   constexpr int BX = WX * TX * 32, BW = WW * TW * 32;
   constexpr int LDS = STAGES * (BX * TileRow<FX>::BYTES + BW * TileRow<MX_E2M1>::BYTES) +
-                      2 * ((BX + 63) / 64 * 64 + BW) * 16;
+                      2 * (BX + BW) * 16;
   const int tx = ai4e_cdiv(m, BX), tw = ai4e_cdiv(n, BW);
   auto* kernel = mx_tile_kernel<FX, DT, WX, WW, TX, TW, STAGES, SHORT>;
   static std::atomic<uint64_t> devices{0};
@@ -330,7 +329,7 @@ int launch_tile(const void* x, const void* xs, const void* w, const void* ws, co
   return hipGetLastError() == hipSuccess ? AI4E_OK : AI4E_ELAUNCH;
 }
 
-// The few-rows kernel: up to 32 rows of x by 128 rows of w per workgroup of 4 waves, a fragment of 32 x 32 each. What
+// The few-rows kernel: up to 32 rows of x by 128 rows of w (at least as many) per workgroup of 4 waves, a fragment of 32 x 32 each. What
 // bounds it is how w comes out of memory: a DMA brings 256 consecutive bytes of 4 rows, four steps of k, since pieces of one
 // step (64 B) of many rows take longer (16 x 32768 x 8192 31.5 us, so 30.2), and past the caches, since a model's weights come by
 // once per token (26.9; weights that a cache still holds 25.5 us, through it 24.0). Such groups of four steps go through a
@@ -731,7 +730,7 @@ int launch_stream(const void* x, const void* xs, const void* w, const void* ws, 
 //   128 x 128 / 64 x 128    512 x 4096 x 4096 (128 / 256 tiles) 17.6 / 12.5     512 x 8192 x 8192 (256 / 512) 38.5 / 45.0
 //   64 x 128 / 64 x 64      256 x 4096 x 4096 (128 / 256 tiles) 12.5 / 10.9     256 x 8192 x 8192 (256 / 512) 26.4 / 33.0
 //   64 x 64 / stream 2      128 x 4096 x 4096 (128 / 256) 10.6 / 7.8            200 x 3000 x 4096 (188 / 329) 11.0 / 11.4
-//   32 x 128 / stream 2     16 x 20480 x 4096 (160 / 320) 15.2 / 17.9           16 x 16384 x 4096 (128 / 256) 13.6 / 10.9
+//   few rows / stream 2     16 x 20480 x 4096 (160 / 320) 14.9 / 17.9           16 x 16384 x 4096 (128 / 256) 13.4 / 11.0
 //   stream 2 / stream 1     64 x 6144 x 4096 (192 / 384) 9.6 / 11.4             64 x 4096 x 4096 (128 / 256) 7.3 / 6.1
 //   stream 1 / slices       1 x 4096 x 4096 5.6 / 4.4                           16 x 4096 x 4096 5.7 / 5.9
 // and with k below 512, where latency counts more than bytes do:
