@@ -10,9 +10,10 @@
 // bits (every logit is the type's lowest value, say) s ends as 0 and the row is summed again from differences x - m.
 //
 // The k best come out of the same pass (logprobs_kernel). A lane also keeps its best chunk (8 consecutive logits; the
-// first one with the lane's maximum). The k-th largest of 256 groups' (maximum, chunk) pairs bounds the k-th best logit
-// from below, so only the k groups at or above it hold candidates: their chunks are read again (from cache), what reaches
-// the bound is put into LDS, and each candidate's rank is the number of candidates before it. Ties go to the lower class.
+// first one with the lane's maximum) and the maxima of SEGMENTS parts of its chunks. The k-th largest of 256 groups'
+// (maximum, chunk) pairs bounds the k-th best logit from below, so only the k groups at or above it hold candidates, and of
+// their parts those that reach it: these are read again, what reaches the bound is put into LDS, and each candidate's rank is
+// the number of candidates before it. Ties go to the lower class.
 // If more candidates come than LDS has room for (their order on the row is adverse), k rounds over the row find one each.
 // Short rows with few alternatives stay in one wave's registers (logprobs_wave_kernel).
 #include <type_traits>
@@ -21,7 +22,7 @@
 
 namespace {
 
-constexpr int KMAX = 64, CAP = 1024, GROUPS = 256;
+constexpr int KMAX = 64, CAP = 1024, GROUPS = 256, SEGMENTS = 8;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LOWEST = -3.402823466e38f;
 constexpr float FAR = -200.f;  // 2^FAR is 0 in 32 bits; keeps 0 * d from being 0 * -inf
@@ -194,7 +195,9 @@ struct Shared {
   float least;           // the bound: a logit over it is a candidate, one equal to it up to chunk `last`
   int last;
   int groups[KMAX];      // the groups at or over the bound
-  int n_groups, n_cand;
+  float part[SEGMENTS][WAVES * 64];  // each lane's maxima of the parts of its chunks
+  uint16_t parts[KMAX * (WAVES * 64 / GROUPS) * SEGMENTS];  // those groups' parts that reach the bound: lane, part
+  int n_groups, n_parts, n_cand;
   uint64_t cand[CAP];    // candidates: the ordered logit, then the class counted down
   float round_value[WAVES];
   int round_index[WAVES];
@@ -251,6 +254,7 @@ __device__ __forceinline__ void find_bound(Shared<WAVES>& sh, int k) {
     sh.least = bound ? unordered(bound) : -INFINITY;
     sh.last = bound ? last : -1;
     sh.n_groups = at;
+    sh.n_parts = 0;
     sh.n_cand = 0;
   }
 }
@@ -266,12 +270,15 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
   __shared__ Shared<WAVES> sh;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int full = c / 8, chunks = (c + 7) / 8;
+  // a lane's chunks, `per` of them T apart, in at most SEGMENTS parts of whole steps
+  const int per = (chunks + T - 1) / T, length = U * ((per + U * SEGMENTS - 1) / (U * SEGMENTS));
   for (long row = blockIdx.x; row < rows; row += gridDim.x) {
     const auto* xr = x + row * ld;
     Label first = {0.f, -1};
     if (wave == 1) first = label<DT>(xr, c, labels, lane, row);
     Stat st = {-INFINITY, 0.f, 0.f};
     int best_chunk = 0;
+    float part = -INFINITY;
     typedef mx_raw8<DT> Pack;
     // N chunks' logits, one rescaling for all
     auto take = [&](auto count, const Pack* q, int at) {
@@ -283,6 +290,7 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
         const float cm = max8(f[u]);
         best_chunk = cm > m ? at + u * T : best_chunk;
         m = fmaxf(m, cm);
+        part = fmaxf(part, cm);
       }
       st = rescaled(st, m);
 #pragma unroll
@@ -296,12 +304,18 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
         for (int u = 0; u < U; ++u) p[u] = mx_load8<DT>(xr + ((step * U + u) * T + tid) * 8l);
       };
       fetch(q, 0);
+      int end = length, p = 0;
       for (int i = 0; i < steps; ++i) {
         Pack next[U];
         if (i + 1 < steps) fetch(next, i + 1);
         take(std::integral_constant<int, U>{}, q, i * U * T + tid);
 #pragma unroll
         for (int u = 0; u < U; ++u) q[u] = next[u];
+        if ((i + 1) * U == end) {
+          sh.part[p++][tid] = part;
+          part = -INFINITY;
+          end += length;
+        }
       }
     }
     for (int at = steps * U * T + tid; at < full; at += T) {
@@ -313,9 +327,11 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
       mx_load8_tail<DT>(xr + full * 8l, c - full * 8, -INFINITY, f);
       const float cm = max8(f);
       best_chunk = cm > st.m ? full : best_chunk;
+      part = fmaxf(part, cm);
       st = rescaled(st, fmaxf(st.m, cm));
       add8(st, f, mu_of(st.m));
     }
+    if (steps * U < per || steps * U % length) sh.part[steps * U / length][tid] = part;  // the last, unfinished part
     float best = st.m;
     const Stat w = wave_join(st);
     if (lane == 0) sh.stat[wave] = w;
@@ -372,10 +388,17 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
       __syncthreads();
       const float least = sh.least;
       const int last = sh.last;
-      const int per = (chunks + T - 1) / T, items = sh.n_groups * MEMBERS * per;
+      const int nparts = (per + length - 1) / length, all_parts = sh.n_groups * MEMBERS * nparts;
+      for (int it = tid; it < all_parts; it += T) {
+        const int g = it / nparts, p = it - g * nparts, from = sh.groups[g / MEMBERS] * MEMBERS + g % MEMBERS;
+        if (sh.part[p][from] >= least) sh.parts[atomicAdd(&sh.n_parts, 1)] = static_cast<uint16_t>(from * SEGMENTS + p);
+      }
+      __syncthreads();
+      const int items = sh.n_parts * length;
       for (int it = tid; it < items; it += T) {
-        const int lanes = it / per, at = sh.groups[lanes / MEMBERS] * MEMBERS + lanes % MEMBERS + (it - lanes * per) * T;
-        if (at >= chunks) continue;
+        const int i = it / length, j = sh.parts[i] % SEGMENTS * length + it - i * length;
+        const int at = sh.parts[i] / SEGMENTS + j * T;
+        if (j >= per || at >= chunks) continue;
         float f[8];
         load_chunk<DT>(xr, at * 8, c, f);
 #pragma unroll
