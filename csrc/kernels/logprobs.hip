@@ -259,10 +259,8 @@ __device__ __forceinline__ void find_bound(Shared<WAVES>& sh, int k) {
   }
 }
 
-// A workgroup of WAVES waves per row. Its loads go through the caches, though 1 GB reads faster past them (7.1 TB/s, 6.3):
-// candidates are read again, and logits are often what the last kernel wrote (333 x 50001 fp32 18.5 us, past the caches
-// 28; 4096 x 131072 bf16 216 and 205).
-template <int DT, int WAVES>
+// A workgroup of WAVES waves per row. PAST: the pass reads past the caches (see launch).
+template <int DT, int WAVES, bool PAST>
 __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_elem<DT>::type* __restrict__ x, long ld,
                                                               long rows, int c, Labels labels, int k, Out out) {
   constexpr int T = WAVES * 64, MEMBERS = T / GROUPS;
@@ -301,7 +299,7 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
       Pack q[U];
       auto fetch = [&](Pack(&p)[U], int step) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) p[u] = mx_load8<DT>(xr + ((step * U + u) * T + tid) * 8l);
+        for (int u = 0; u < U; ++u) p[u] = mx_load8<DT, PAST>(xr + ((step * U + u) * T + tid) * 8l);
       };
       fetch(q, 0);
       int end = length, p = 0;
@@ -541,8 +539,12 @@ void launch(const void* x, long ld, long rows, int c, const Labels& labels, int 
   // 16 waves per row where there are too few rows to fill the CUs with 4 (1 x 131072: 17.4 us against 22.8, 256 x 131072
   // 24.8 against 40.4); with more rows their phases cost more (512 x 131072 45.7 against 45.3, 333 x 50001 fp32 25.8
   // against 23.5, 1024 x 32768 47.6 against 25.2)
-  if (rows <= 256 && c >= 8192) GO(grid, 1024, logprobs_kernel<DT, 16>);
-  else GO(grid, 256, logprobs_kernel<DT, 4>);
+  if (rows <= 256 && c >= 8192) GO(grid, 1024, logprobs_kernel<DT, 16, false>);
+  // Logits are often what the last kernel wrote, so they are read through the caches (333 x 50001 fp32 18.5 us, past them
+  // 28). No cache holds 512 MB of them: 16-bit ones then come faster past the caches (4096 x 131072 212 us, past them 193),
+  // 32-bit ones do not (2048 x 131072 195, 199).
+  else if (DT != MX_F32 && rows * c >= (256l << 20)) GO(grid, 256, logprobs_kernel<DT, 4, DT != MX_F32>);
+  else GO(grid, 256, logprobs_kernel<DT, 4, false>);
 #undef GO
 }
 

@@ -49,11 +49,14 @@ struct mx_raw8 {
   mx_i32x4_t v[DT == MX_F32 ? 2 : 1];
 };
 
-template <int DT>
+template <int DT, bool PAST = false>
 __device__ __forceinline__ mx_raw8<DT> mx_load8(const typename mx_elem<DT>::type* p) {
   mx_raw8<DT> w;
 #pragma unroll
-  for (int i = 0; i < (DT == MX_F32 ? 2 : 1); ++i) w.v[i] = reinterpret_cast<const mx_i32x4_t*>(p)[i];
+  for (int i = 0; i < (DT == MX_F32 ? 2 : 1); ++i) {
+    const auto* q = reinterpret_cast<const mx_i32x4_t*>(p) + i;
+    w.v[i] = PAST ? __builtin_nontemporal_load(q) : *q;
+  }
   return w;
 }
 

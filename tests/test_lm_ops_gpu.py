@@ -345,6 +345,26 @@ def test_logprobs_more_candidates_than_room(c):
     check_logprobs(x[:8].contiguous(), labels[:8], 20)
 
 
+@pytest.mark.parametrize("dtype,rows,c,k", [(torch.bfloat16, 2100, 130001, 20), (torch.float16, 9000, 30000, 64)])
+def test_logprobs_more_than_caches_hold(dtype, rows, c, k):
+    """Rows of a call of over 512 MB, against the same rows called by themselves and a few of them against the oracle."""
+    g = torch.Generator(DEV).manual_seed(c)
+    x = torch.empty(rows, c, device=DEV, dtype=dtype).normal_(0, 3, generator=g)
+    x[0, 100:] = -math.inf
+    x[1] = 1.0
+    x[2] = -math.inf
+    x[rows - 1, ::3] = torch.finfo(dtype).min
+    labels = torch.randint(0, c, (rows,), generator=g, device=DEV)
+    got = label_logprobs(x, labels, k)
+    for at in (0, rows // 2, rows - 300):
+        part = label_logprobs(x[at:at + 300], labels[at:at + 300], k)
+        assert torch.equal(got.top_idx[at:at + 300], part.top_idx)
+        for a, b in ((got.logp, part.logp), (got.entropy, part.entropy), (got.top_logp, part.top_logp)):
+            assert torch.equal(a[at:at + 300], b)
+    pick = [0, 1, 2, rows // 2, rows - 1]
+    check_logprobs(x[pick].cpu(), labels[pick].cpu(), k)
+
+
 def test_logprobs_not_finite_rows():
     for c in (500, 30000):
         x = torch.randn(6, c, generator=gen(c))
