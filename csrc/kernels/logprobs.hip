@@ -536,9 +536,9 @@ void launch(const void* x, long ld, long rows, int c, const Labels& labels, int 
     return;
   }
   const long grid = rows < (1 << 20) ? rows : (1 << 20);
-  // 16 waves per row where there are too few rows to fill the CUs with 4 (1 x 131072: 17.4 us against 22.8, 256 x 131072
-  // 24.8 against 40.4); with more rows their phases cost more (512 x 131072 45.7 against 45.3, 333 x 50001 fp32 25.8
-  // against 23.5, 1024 x 32768 47.6 against 25.2)
+  // 16 waves per row where there are too few rows to fill the CUs with 4 (1 x 131072: 14.6 us against 18.3, 256 x 131072
+  // 24.3 against 30.4, 256 x 9000 12.1 against 11.2); with more rows their phases cost more (512 x 131072 47.2 against 45.7,
+  // 333 x 50001 fp32 26.2 against 18.3, 1024 x 32768 48.9 against 23.8)
   if (rows <= 256 && c >= 8192) GO(grid, 1024, logprobs_kernel<DT, 16, false>);
   // Logits are often what the last kernel wrote, so they are read through the caches (333 x 50001 fp32 18.5 us, past them
   // 28). No cache holds 512 MB of them: 16-bit ones then come faster past the caches (4096 x 131072 212 us, past them 193),
