@@ -6,8 +6,10 @@
 //
 // One pass: a lane keeps its maximum, s and t of the elements it has seen and rescales s and t when the maximum grows, so
 // a logit is read once. The pass works in base 2, s = sum 2^d and t = sum 2^d d with d = x log2 e - mu in one fused
-// operation, mu the rounded m log2 e: what mu lost is put back at the end. -inf gives 2^d = 0. Where m log2 e leaves 32
-// bits (every logit is the type's lowest value, say) s ends as 0 and the row is summed again from differences x - m.
+// operation, mu the rounded m log2 e: what mu lost, at most 2^-8, is put back at the end. -inf gives 2^d = 0. From
+// |m| = 2^16 on mu would lose more, up to what 2^d cannot hold: there it lies over m log2 e, so that no d is over 0 and a
+// lane that has seen nothing but such a mask adds 0 to its row, and a row whose maximum lies there is summed again from
+// differences x - m.
 //
 // The k best come out of the same pass (logprobs_kernel). A lane also keeps its best chunk (8 consecutive logits; the
 // first one with the lane's maximum) and the maxima of SEGMENTS parts of its chunks. The k-th largest of 256 groups'
@@ -25,6 +27,7 @@ namespace {
 constexpr int KMAX = 64, CAP = 1024, GROUPS = 256, SEGMENTS = 8;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LOWEST = -3.402823466e38f;
+constexpr float OUTER = 65536.f;  // logits from here on are summed from differences (fp16 has none)
 constexpr float FAR = -200.f;  // 2^FAR is 0 in 32 bits; keeps 0 * d from being 0 * -inf
 
 // the largest logit (-inf: none yet) and the sums relative to it
@@ -32,13 +35,19 @@ struct Stat {
   float m, s, t;
 };
 
-__device__ __forceinline__ float mu_of(float m) { return fmaxf(m * LOG2E, LOWEST); }
+__device__ __forceinline__ float mu_of(float m) {
+  const float p = m * LOG2E, a = fabsf(m);
+  return fmaxf(a < OUTER ? p : fmaf(a, 0x1p-20f, p), LOWEST);  // 2^-20 m is over the two roundings of m log2 e
+}
 
-// v's sums (base 2) relative to a maximum m >= v.m
-__device__ __forceinline__ Stat rescaled(const Stat& v, float m) {
-  const float d = mu_of(v.m) - mu_of(m), f = __builtin_amdgcn_exp2f(d);
+// v's sums (base 2), taken relative to mu, relative to a maximum m >= v.m, whose reference is to_mu
+__device__ __forceinline__ Stat rescaled(const Stat& v, float mu, float m, float to_mu) {
+  // the minimum only makes a number of inf - inf (both references are over 32 bits: the sums are 0); at m = -OUTER, where
+  // mu steps up, the difference may be as large as 2^-4
+  const float d = fminf(mu - to_mu, 1.f), f = __builtin_amdgcn_exp2f(d);
   return {m, v.s * f, f * (v.t + fmaxf(d, FAR) * v.s)};
 }
+__device__ __forceinline__ Stat rescaled(const Stat& v, float m) { return rescaled(v, mu_of(v.m), m, mu_of(m)); }
 
 // lane i's value from lane i ^ 1, i ^ 2, 7 - i of 8, 15 - i of 16: four steps that join 16 lanes
 template <int STEP>
@@ -275,6 +284,7 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
     Label first = {0.f, -1};
     if (wave == 1) first = label<DT>(xr, c, labels, lane, row);
     Stat st = {-INFINITY, 0.f, 0.f};
+    float mu = LOWEST;  // st's reference, mu_of(st.m)
     int best_chunk = 0;
     float part = -INFINITY;
     typedef mx_raw8<DT> Pack;
@@ -290,9 +300,11 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
         m = fmaxf(m, cm);
         part = fmaxf(part, cm);
       }
-      st = rescaled(st, m);
+      const float to_mu = mu_of(m);
+      st = rescaled(st, mu, m, to_mu);
+      mu = to_mu;
 #pragma unroll
-      for (int u = 0; u < N; ++u) add8(st, f[u], mu_of(m));
+      for (int u = 0; u < N; ++u) add8(st, f[u], mu);
     };
     const int steps = full / (U * T);
     if (steps > 0) {
@@ -360,8 +372,8 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
       all.s += r.s;
       all.t += r.t;
     }
-    const bool again = all.s == 0.f && all.m > -INFINITY;
-    if (again) {  // m log2 e is out of range
+    const bool again = fabsf(all.m) >= OUTER && fabsf(all.m) < INFINITY;
+    if (again) {
       Stat d = {all.m, 0.f, 0.f};
       for (int at = tid; at < chunks; at += T) {
         float f[8];
@@ -373,7 +385,7 @@ __global__ __launch_bounds__(WAVES * 64) void logprobs_kernel(const typename mx_
       __syncthreads();  // every wave has read the first sums
       if (lane == 0) sh.stat[wave] = d;
       __syncthreads();
-      all.t = 0.f;
+      all.s = all.t = 0.f;
 #pragma unroll
       for (int i = 0; i < WAVES; ++i) {
         all.s += sh.stat[i].s;
