@@ -764,10 +764,11 @@ int launch(const void* x, const void* xs, const void* w, const void* ws, const v
 // bias [n] fp32 or null; y [m, n] of type dt (0 bf16, 1 fp16, 2 fp32). kp is a multiple of 128.
 AI4E_API int ai4e_mx_linear(const void* x, const void* xs, int fx, const void* w, const void* ws, const void* bias,
                             int m, int n, int kp, void* y, int dt, hipStream_t s) {
-  if (!x || !xs || !w || !ws || !y || m < 0 || n <= 0 || kp <= 0 || kp % MX_ALIGN || fx < 0 || fx > 1 || dt < 0 || dt > 2 ||
+  if (m < 0 || n <= 0 || kp <= 0 || kp % MX_ALIGN || fx < 0 || fx > 1 || dt < 0 || dt > 2 ||
       kp > (1 << 23) || n > (1 << 30) || m > (1 << 30) || static_cast<long>(ai4e_cdiv(m, 128)) * ai4e_cdiv(n, 128) > (1L << 22))
     return AI4E_EINVAL;
-  if (m == 0) return AI4E_OK;
+  if (m == 0) return AI4E_OK;  // tensors without elements have no memory
+  if (!x || !xs || !w || !ws || !y) return AI4E_EINVAL;
 #define GO(FX, DT) return launch<FX, DT>(x, xs, w, ws, bias, m, n, kp, y, s)
   if (fx == MX_E4M3) {
     if (dt == MX_BF16) GO(MX_E4M3, MX_BF16);

@@ -104,8 +104,8 @@ __global__ __launch_bounds__(THREADS) void dequantize_kernel(const uint8_t* __re
 }
 
 // a launch has fewer than 2^32 threads
-bool bad_shape(const void* a, const void* b, const void* c, long rows, int k) {
-  return !a || !b || !c || rows < 0 || k <= 0 || k > (1 << 30) ||
+bool bad_shape(long rows, int k) {
+  return rows < 0 || k <= 0 || k > (1 << 30) ||
          rows > ((1L << 32) - THREADS) * PER / (static_cast<long>(ai4e_cdiv(k, MX_ALIGN)) * (MX_ALIGN / 8));
 }
 
@@ -123,8 +123,9 @@ bool bad_shape(const void* a, const void* b, const void* c, long rows, int k) {
 // data [rows, kp] (fmt 0, e4m3) or [rows, kp / 2] (fmt 1, e2m1), scale [rows, kp / 32].
 AI4E_API int ai4e_mx_quantize(const void* x, long ldx, long rows, int k, int dt, int fmt, void* data, void* scale,
                               hipStream_t s) {
-  if (dt < 0 || dt > 2 || fmt < 0 || fmt > 1 || bad_shape(x, data, scale, rows, k) || ldx < k) return AI4E_EINVAL;
-  if (rows == 0) return AI4E_OK;
+  if (dt < 0 || dt > 2 || fmt < 0 || fmt > 1 || bad_shape(rows, k) || ldx < k) return AI4E_EINVAL;
+  if (rows == 0) return AI4E_OK;  // tensors without elements have no memory
+  if (!x || !data || !scale) return AI4E_EINVAL;
   const int kp = ai4e_cdiv(k, MX_ALIGN) * MX_ALIGN;
   const dim3 grid(ai4e_cdiv(rows * (kp / 8), THREADS * PER)), block(THREADS);
 #define DO(DT, FMT)                                                                                               \
@@ -138,8 +139,9 @@ AI4E_API int ai4e_mx_quantize(const void* x, long ldx, long rows, int k, int dt,
 // the values that codes stand for: y [rows, k] contiguous, of type dt
 AI4E_API int ai4e_mx_dequantize(const void* data, const void* scale, long rows, int k, int dt, int fmt, void* y,
                                 hipStream_t s) {
-  if (dt < 0 || dt > 2 || fmt < 0 || fmt > 1 || bad_shape(data, scale, y, rows, k)) return AI4E_EINVAL;
+  if (dt < 0 || dt > 2 || fmt < 0 || fmt > 1 || bad_shape(rows, k)) return AI4E_EINVAL;
   if (rows == 0) return AI4E_OK;
+  if (!data || !scale || !y) return AI4E_EINVAL;
   const int kp = ai4e_cdiv(k, MX_ALIGN) * MX_ALIGN;
   const dim3 grid(ai4e_cdiv(rows * (kp / 8), THREADS * PER)), block(THREADS);
 #define DO(DT, FMT)                                                                                                   \

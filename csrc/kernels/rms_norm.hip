@@ -146,10 +146,10 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_mx8_kernel
 // hout [rows, c] of type dt (or null); data [rows, cp], scale [rows, cp / 32], cp = c up to a multiple of 128.
 AI4E_API int ai4e_rms_norm_mx8(const void* x, long ldx, const void* residual, long ldr, const void* gamma, float eps,
                                long rows, int c, int dt, void* hout, void* data, void* scale, hipStream_t s) {
-  if (!x || !gamma || !data || !scale || c <= 0 || c > (1 << 30) || rows < 0 || dt < 0 || dt > 2 || ldx < c ||
-      (residual && ldr < c) || !(eps > 0.f))
+  if (c <= 0 || c > (1 << 30) || rows < 0 || dt < 0 || dt > 2 || ldx < c || (residual && ldr < c) || !(eps > 0.f))
     return AI4E_EINVAL;
-  if (rows == 0) return AI4E_OK;
+  if (rows == 0) return AI4E_OK;  // tensors without elements have no memory
+  if (!x || !gamma || !data || !scale) return AI4E_EINVAL;
   const int cp = ai4e_cdiv(c, MX_ALIGN) * MX_ALIGN;
 #define GO(DT, LANES, CH)                                                                                        \
   {                                                                                                              \

@@ -1,0 +1,24 @@
+"""Language-model operators at the edges of what their documents allow, without a GPU."""
+import pytest
+
+from aiforearth_api_platform_amd.ops import _ext
+
+
+def kernels():
+    if not _ext.available():
+        pytest.skip("kernel library not built")
+    return _ext.lib()
+
+
+def test_c_entries_take_no_rows_at_null():
+    """A tensor without elements has no memory: every pointer is null, and there is nothing to do (no GPU is touched)."""
+    lib = kernels()
+    assert lib.ai4e_mx_quantize(None, 40, 0, 40, 0, 0, None, None, None) == 0
+    assert lib.ai4e_mx_dequantize(None, None, 0, 40, 0, 1, None, None) == 0
+    assert lib.ai4e_rms_norm_mx8(None, 40, None, 0, 16, 1e-6, 0, 40, 0, None, None, None, None) == 0
+    assert lib.ai4e_label_logprobs(None, 40, 0, 40, 0, None, 0, 0, 5, None, None, None, None, None) == 0
+    assert lib.ai4e_mx_linear(None, None, 0, 16, 16, None, 0, 8, 128, None, 0, None) == 0
+    # what else is wrong with such a call is still refused
+    assert lib.ai4e_mx_quantize(None, 40, 0, 41, 0, 0, None, None, None) == 1
+    assert lib.ai4e_rms_norm_mx8(None, 40, None, 0, 16, 0.0, 0, 40, 0, None, None, None, None) == 1
+    assert lib.ai4e_mx_linear(None, None, 0, 16, 16, None, 0, 8, 64, None, 0, None) == 1

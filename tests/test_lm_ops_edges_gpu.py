@@ -4,7 +4,10 @@ import math
 import pytest
 import torch
 
+from aiforearth_api_platform_amd.ops import mx
 from aiforearth_api_platform_amd.ops.head import label_logprobs
+from aiforearth_api_platform_amd.ops.mx import mx_dequantize, mx_linear, mx_quantize
+from aiforearth_api_platform_amd.ops.norm import rms_norm_mx8
 from test_lm_ops_gpu import DEV, check_logprobs, gen
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +80,22 @@ def test_logprobs_not_finite_among_large_logits():
             # 32-bit sums of up to c / 256 + 64 equal terms, and a logarithm
             for r, n in ((2, 100), (3, c)):
                 assert abs(got.logp[r].item() + math.log(n)) <= (c / 256 + 64) * 2.0 ** -24 + math.log(n) * 2.0 ** -22
+
+
+@pytest.mark.parametrize("shape", [(0, 40), (0, 3000), (2, 0, 600), (0, 0, 128)])
+def test_no_rows(shape):
+    """A batch without rows goes through every operator, alone and in their order."""
+    lead, c = shape[:-1], shape[-1]
+    x = torch.empty(shape, device=DEV)
+    w = mx_quantize(torch.randn(30, c, device=DEV))
+    for fmt in ("e2m1", "e4m3"):
+        q = mx_quantize(x.bfloat16(), fmt)
+        assert q.shape == shape and q.scale.shape == (*lead, mx.padded(c) // 32)
+        assert mx_dequantize(q).shape == shape
+        assert mx_linear(q, w).shape == (*lead, 30)
+    for residual in (None, x):
+        q, h = rms_norm_mx8(x, torch.ones(c, device=DEV), residual)
+        assert q.shape == shape and (h is None if residual is None else h.shape == shape)
+        y = mx_linear(q, w)
+        got = label_logprobs(y, torch.empty(lead, dtype=torch.int64, device=DEV), 5)
+        assert got.logp.shape == got.entropy.shape == lead and got.top_idx.shape == got.top_logp.shape == (*lead, 5)
