@@ -162,8 +162,8 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
         raise ValueError(f"rms_norm_mx8: gamma is a floating tensor of {c} values")
     if gamma.get_device() != index or (residual is not None and residual.get_device() != index):
         raise ValueError("rms_norm_mx8: x, gamma and residual have to be on one device")
-    if not eps > 0:
-        raise ValueError("rms_norm_mx8: eps has to be positive")
+    if not eps >= 2.0 ** -149:  # from there on a row's factor is a 32-bit number, whatever the row holds
+        raise ValueError("rms_norm_mx8: eps has to be positive, 2^-149 or more")
     _ext.refuse_grad("rms_norm_mx8", x, gamma, residual)
     if _ext.backend_for(x) != "hip":
         h = x.float() if residual is None else x.float() + residual.float()

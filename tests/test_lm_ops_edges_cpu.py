@@ -1,7 +1,9 @@
 """Language-model operators at the edges of what their documents allow, without a GPU."""
 import pytest
+import torch
 
 from aiforearth_api_platform_amd.ops import _ext
+from aiforearth_api_platform_amd.ops.norm import rms_norm_mx8
 
 
 def kernels():
@@ -22,3 +24,9 @@ def test_c_entries_take_no_rows_at_null():
     assert lib.ai4e_mx_quantize(None, 40, 0, 41, 0, 0, None, None, None) == 1
     assert lib.ai4e_rms_norm_mx8(None, 40, None, 0, 16, 0.0, 0, 40, 0, None, None, None, None) == 1
     assert lib.ai4e_mx_linear(None, None, 0, 16, 16, None, 0, 8, 64, None, 0, None) == 1
+
+
+@pytest.mark.parametrize("eps", [0.0, -1e-6, 1e-46, float("nan")])
+def test_rms_norm_refuses_an_eps_that_32_bits_do_not_hold(eps):
+    with pytest.raises(ValueError):
+        rms_norm_mx8(torch.ones(2, 64), torch.ones(64), eps=eps)

@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+import lm_oracle as oracle
 from aiforearth_api_platform_amd.ops import mx
 from aiforearth_api_platform_amd.ops.head import label_logprobs
 from aiforearth_api_platform_amd.ops.mx import mx_dequantize, mx_linear, mx_quantize
@@ -99,3 +100,19 @@ def test_no_rows(shape):
         y = mx_linear(q, w)
         got = label_logprobs(y, torch.empty(lead, dtype=torch.int64, device=DEV), 5)
         assert got.logp.shape == got.entropy.shape == lead and got.top_idx.shape == got.top_logp.shape == (*lead, 5)
+
+
+@pytest.mark.parametrize("c", [64, 3000, 20000])
+def test_rms_norm_eps_is_not_rounded(c):
+    """Where eps outweighs the squares, y is x / sqrt(eps) * gamma. 1.1875 is the border between 1.125 and 1.25 and falls to
+    the latter; what 32 bits do not hold of this eps takes y below it."""
+    eps = 2.0 ** -20 * (1 + 2.0 ** -25)
+    x = torch.full((3, c), 2.0 ** -40)
+    x[1] = -x[1]
+    gamma = torch.full((c,), 1.1875)
+    q, _ = rms_norm_mx8(x.to(DEV), gamma.to(DEV), None, eps)
+    want = oracle.mx_values(oracle.rms_norm(x, gamma, None, eps), "e4m3")
+    assert want[0].eq(1.125 * 2.0 ** -30).all() and torch.equal(mx_dequantize(q).cpu().double(), want)
+    q, _ = rms_norm_mx8(x * 2.0 ** -30, gamma, None, 2.0 ** -149)
+    p, _ = rms_norm_mx8((x * 2.0 ** -30).to(DEV), gamma.to(DEV), None, 2.0 ** -149)
+    assert torch.equal(mx_dequantize(p).cpu(), mx_dequantize(q))
