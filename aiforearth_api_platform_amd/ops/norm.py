@@ -146,6 +146,15 @@ def upsample2x_nhwc(x: torch.Tensor, out: Optional[torch.Tensor] = None, out_cof
     return out
 
 
+def _rounded_to_odd(y: torch.Tensor) -> torch.Tensor:
+    """64-bit ``y`` in 32 bits, of its two neighbours the one with an odd significand: a border of a shorter format, which
+    is even, is met by an exact value only, so that rounding to that format is the only one."""
+    f = y.float()
+    bits, wide = f.view(torch.int32), f.double()
+    move = (wide != y) & torch.isfinite(f) & (bits & 1 == 0)
+    return torch.where(move, torch.where(y.abs() > wide.abs(), bits + 1, bits - 1), bits).view(torch.float32)
+
+
 def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.Tensor] = None,
                  eps: float = 1e-6) -> Tuple[mx.MxTensor, Optional[torch.Tensor]]:
     """``h = x + residual``; ``h / sqrt(mean(h^2) + eps) * gamma`` over the last axis, as MX e4m3 activations for
@@ -169,7 +178,7 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
         h = x.float() if residual is None else x.float() + residual.float()
         h64 = h.double() if residual is None else torch.where(h.isfinite(), x.double() + residual.double(), h.double())
         y = h64 / torch.sqrt(h64.square().mean(-1, keepdim=True) + eps) * gamma.double()
-        return mx.quantize_reference(y.float(), "e4m3"), None if residual is None else h.to(x.dtype)
+        return mx.quantize_reference(_rounded_to_odd(y), "e4m3"), None if residual is None else h.to(x.dtype)
     q = mx.empty(shape[:-1], c, "e4m3", x.device)
     h = None if residual is None else mx.new(shape, x.dtype, x.device)
     g32 = gamma if gamma.dtype == torch.float32 and gamma.is_contiguous() else gamma.to(torch.float32).contiguous()

@@ -2,7 +2,9 @@
 import pytest
 import torch
 
+import lm_oracle as oracle
 from aiforearth_api_platform_amd.ops import _ext
+from aiforearth_api_platform_amd.ops.mx import mx_dequantize
 from aiforearth_api_platform_amd.ops.norm import rms_norm_mx8
 
 
@@ -30,3 +32,17 @@ def test_c_entries_take_no_rows_at_null():
 def test_rms_norm_refuses_an_eps_that_32_bits_do_not_hold(eps):
     with pytest.raises(ValueError):
         rms_norm_mx8(torch.ones(2, 64), torch.ones(64), eps=eps)
+
+
+def test_rms_norm_reference_rounds_once():
+    """y lies below the border 1.1875 of 1.125 and 1.25 by less than 32 bits hold: it becomes 1.125."""
+    eps = 2.0 ** -20 * (1 + 2.0 ** -25)
+    x, gamma = torch.full((2, 40), 2.0 ** -40), torch.full((40,), 1.1875)
+    x[1] *= -1
+    want = oracle.mx_values(oracle.rms_norm(x, gamma, None, eps), "e4m3")
+    assert want[0].eq(1.125 * 2.0 ** -30).all()
+    assert torch.equal(mx_dequantize(rms_norm_mx8(x, gamma, None, eps)[0]).double(), want)
+    # above the border between 1 and 1.125, which falls to 1; at one it stays there
+    gamma[:] = 1.0625
+    for e, value in ((2.0 ** -20 * (1 - 2.0 ** -25), 1.125), (2.0 ** -20, 1.0)):
+        assert mx_dequantize(rms_norm_mx8(x, gamma, None, e)[0])[0].eq(value * 2.0 ** -30).all()
