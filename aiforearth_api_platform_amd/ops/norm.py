@@ -160,7 +160,8 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
     """``h = x + residual``; ``h / sqrt(mean(h^2) + eps) * gamma`` over the last axis, as MX e4m3 activations for
     ``mx.mx_linear`` (csrc/kernels/rms_norm.hip). ``x`` and ``residual`` [..., C] in bf16, fp16 or fp32 (rows may be
     strided), ``gamma`` [C] (kept in float32 by a caller that wants no cast per call). Returns the MxTensor and ``h`` in
-    x's type, for the next residual (None without ``residual``); the norm is taken of the sum before that rounding."""
+    x's type, for the next residual (None without ``residual``); the norm is taken of the sum before that rounding: of the
+    32-bit sum of 16-bit rows, of the exact sum of 32-bit ones."""
     c = x.shape[-1] if x.dim() else 0
     if x.dtype not in mx.DTYPE_CODE or not 0 < c <= mx.MAX_WIDTH:
         raise ValueError("rms_norm_mx8 expects bfloat16, float16 or float32 with a last axis of 1 to 2^30 values")
@@ -176,7 +177,9 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
     _ext.refuse_grad("rms_norm_mx8", x, gamma, residual)
     if _ext.backend_for(x) != "hip":
         h = x.float() if residual is None else x.float() + residual.float()
-        h64 = h.double() if residual is None else torch.where(h.isfinite(), x.double() + residual.double(), h.double())
+        h64 = h.double()
+        if residual is not None and x.dtype == torch.float32:  # what the sum's rounding lost, as the kernel has it
+            h64 = torch.where(h.isfinite(), x.double() + residual.double(), h.double())
         y = h64 / torch.sqrt(h64.square().mean(-1, keepdim=True) + eps) * gamma.double()
         return mx.quantize_reference(_rounded_to_odd(y), "e4m3"), None if residual is None else h.to(x.dtype)
     q = mx.empty(shape[:-1], c, "e4m3", x.device)

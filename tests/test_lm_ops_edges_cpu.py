@@ -46,3 +46,11 @@ def test_rms_norm_reference_rounds_once():
     gamma[:] = 1.0625
     for e, value in ((2.0 ** -20 * (1 - 2.0 ** -25), 1.125), (2.0 ** -20, 1.0)):
         assert mx_dequantize(rms_norm_mx8(x, gamma, None, e)[0])[0].eq(value * 2.0 ** -30).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rms_norm_reference_takes_the_kernels_sums(dtype):
+    """Sums of 16-bit rows are 32-bit numbers: 4.25 + 2^-23 is 4.25, the border of 4 and 4.5, and falls to 4."""
+    x, r = torch.full((2, 64), 4.25, dtype=dtype), torch.full((2, 64), 2.0 ** -23, dtype=dtype)
+    q, h = rms_norm_mx8(x, torch.ones(64), r, 2.0 ** 40)
+    assert mx_dequantize(q).eq(4 * 2.0 ** -20).all() and h.eq(4.25).all()

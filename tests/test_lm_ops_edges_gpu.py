@@ -116,3 +116,19 @@ def test_rms_norm_eps_is_not_rounded(c):
     q, _ = rms_norm_mx8(x * 2.0 ** -30, gamma, None, 2.0 ** -149)
     p, _ = rms_norm_mx8((x * 2.0 ** -30).to(DEV), gamma.to(DEV), None, 2.0 ** -149)
     assert torch.equal(mx_dequantize(p).cpu(), mx_dequantize(q))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("c", [64, 500, 3000, 8192, 20000])
+def test_rms_norm_of_sums_past_32_bits(dtype, c):
+    """x + residual lies above 4.25, of which 1.0625 is the border between 1 and 1.125, by less than 32 bits hold. Sums of
+    16-bit rows are 32-bit numbers (4.25, which falls to 4); of 32-bit rows what the sum lost counts (4.5). So on both devices."""
+    x, r = torch.full((2, c), 4.25), torch.full((2, c), 2.0 ** -23)
+    r[1] = 0
+    eps = 2.0 ** 40  # y is the sum times 2^-20, less 2^-37 of it
+    x, r, gamma = x.to(dtype), r.to(dtype), torch.ones(c)
+    first = 4.5 if dtype == torch.float32 else 4.0
+    want = torch.tensor([first, 4.0])[:, None].expand(2, c) * 2.0 ** -20
+    for dev in ("cpu", DEV):
+        q, h = rms_norm_mx8(x.to(dev), gamma.to(dev), r.to(dev), eps)
+        assert torch.equal(mx_dequantize(q).cpu(), want) and h.eq(4.25).all(), dev
