@@ -60,6 +60,8 @@ def label_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, 
         if shape != lead and (len(shape) == 0 or shape[:-1] != lead):
             raise ValueError(f"label_logprobs: labels {tuple(shape)} fit no logits {tuple(logits.shape)}")
         n_labels = 1 if shape == lead else shape[-1]
+        if n_labels > mx.MAX_WIDTH:
+            raise ValueError("label_logprobs: a row has up to 2^30 labels")
     _ext.refuse_grad("label_logprobs", logits)
     if _ext.backend_for(logits) != "hip":
         return _label_logprobs_reference(logits, labels, n_labels, k)

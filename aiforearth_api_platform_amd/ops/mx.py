@@ -130,6 +130,11 @@ def dequantize_reference(q: MxTensor) -> torch.Tensor:
     return (v.reshape(*code.shape, BLOCK) * s[..., None]).reshape(v.shape)[..., :q.k]
 
 
+def _check_rows(name: str, rows: int, k: int) -> None:
+    if rows * (padded(k) // 8) > (1 << 33) - 512:  # a launch has fewer than 2^32 threads, of 16 values each
+        raise ValueError(f"{name}: rows of {k} are taken up to {((1 << 33) - 512) // (padded(k) // 8)} at once, not {rows}")
+
+
 def mx_quantize(x: torch.Tensor, fmt: str = "e2m1") -> MxTensor:
     """``[..., K]`` (bf16, fp16 or fp32; rows may be strided) -> MxTensor of ``fmt`` ("e2m1" or "e4m3")."""
     if fmt not in FMT_CODE:
@@ -137,6 +142,7 @@ def mx_quantize(x: torch.Tensor, fmt: str = "e2m1") -> MxTensor:
     if x.dtype not in DTYPE_CODE or x.dim() < 1 or not 0 < x.shape[-1] <= MAX_WIDTH:
         raise ValueError("mx_quantize expects bfloat16, float16 or float32 with a last axis of 1 to 2^30 values")
     _ext.refuse_grad("mx_quantize", x)
+    _check_rows("mx_quantize", x.numel() // x.shape[-1], x.shape[-1])
     if _ext.backend_for(x) != "hip":
         return quantize_reference(x, fmt)
     k = x.shape[-1]
@@ -152,6 +158,7 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
     check("mx_dequantize", q)
     if dtype not in DTYPE_CODE:
         raise ValueError("mx_dequantize gives bfloat16, float16 or float32")
+    _check_rows("mx_dequantize", q.scale.numel() // q.scale.shape[-1], q.k)
     if _ext.backend_for(q.data) != "hip":
         return dequantize_reference(q).to(dtype)
     y = new(q.shape, dtype, q.data.device)
@@ -159,6 +166,13 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
         _ext.call_on(y.get_device(), "ai4e_mx_dequantize", q.data.data_ptr(), q.scale.data_ptr(), y.numel() // q.k, q.k,
                      DTYPE_CODE[dtype], FMT_CODE[q.fmt], y.data_ptr())
     return y
+
+
+def _linear_fits(m: int, n: int, kp: int) -> bool:
+    """Whether a launch holds ``m`` rows of ``kp`` stored values by ``n`` outputs (``fits`` in csrc/kernels/mx_linear.hip)."""
+    rows, cols = -(-m // 128), -(-n // 128)
+    slices = kp < 512 and (m <= 32 or n < 4)
+    return kp <= 1 << 23 and rows * cols <= 1 << 22 and not (slices and -(-m // 32) * -(-n // 64) >= 1 << 23)
 
 
 def mx_linear(x: MxTensor, w: MxTensor, bias: Optional[torch.Tensor] = None,
@@ -184,6 +198,10 @@ def mx_linear(x: MxTensor, w: MxTensor, bias: Optional[torch.Tensor] = None,
     n = w.data.shape[0]
     if bias is not None and (tuple(bias.shape) != (n,) or not bias.is_floating_point()):
         raise ValueError(f"mx_linear: bias is a floating tensor of {n} values")
+    m = scale.numel() // scale.shape[-1]
+    if not _linear_fits(m, n, padded(k)):
+        raise ValueError(f"mx_linear: {m} rows of {k} by {n} outputs are more than a launch holds (k up to 2^23, 2^22 tiles of "
+                         "128 rows by 128 outputs)")
     index = data.get_device()
     if w.data.get_device() != index or (bias is not None and bias.get_device() != index):
         raise ValueError("mx_linear: x, w and bias have to be on one device")
@@ -195,5 +213,5 @@ def mx_linear(x: MxTensor, w: MxTensor, bias: Optional[torch.Tensor] = None,
     if y.numel():
         b32 = None if bias is None else bias.to(torch.float32).contiguous()
         _ext.call_on(index, "ai4e_mx_linear", data.data_ptr(), scale.data_ptr(), FMT_CODE[fmt], w.data.data_ptr(),
-                     w.scale.data_ptr(), _ext.ptr(b32), y.numel() // n, n, padded(k), y.data_ptr(), DTYPE_CODE[out_dtype])
+                     w.scale.data_ptr(), _ext.ptr(b32), m, n, padded(k), y.data_ptr(), DTYPE_CODE[out_dtype])
     return y

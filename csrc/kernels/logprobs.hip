@@ -567,7 +567,8 @@ void launch(const void* x, long ld, long rows, int c, const Labels& labels, int 
 AI4E_API int ai4e_label_logprobs(const void* logits, long ld, long rows, int c, int dt, const void* labels, int wide,
                                  int n_labels, int k, void* logp, void* entropy, void* top_idx, void* top_logp,
                                  hipStream_t s) {
-  if (c <= 0 || c > (1 << 30) || ld < c || rows < 0 || dt < 0 || dt > 2 || k < 0 || k > KMAX || k > c || n_labels < 0)
+  if (c <= 0 || c > (1 << 30) || ld < c || rows < 0 || dt < 0 || dt > 2 || k < 0 || k > KMAX || k > c || n_labels < 0 ||
+      n_labels > (1 << 30))
     return AI4E_EINVAL;
   if (rows == 0) return AI4E_OK;  // tensors without elements have no memory
   if (!logits || !entropy || (n_labels && (!labels || !logp)) || (k && (!top_idx || !top_logp))) return AI4E_EINVAL;

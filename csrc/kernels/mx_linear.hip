@@ -562,7 +562,6 @@ template <int FX, int DT, int MT, int NT>
 int launch_slice(const void* x, const void* xs, const void* w, const void* ws, const void* bias, int m, int n, int kp, void* y,
                  hipStream_t s) {
   const int tm = ai4e_cdiv(m, 16 * MT);
-  if (static_cast<long>(tm) * ai4e_cdiv(n, 16 * NT) >= 1L << 23) return AI4E_EINVAL;  // a launch has fewer than 2^32 threads
   hipLaunchKernelGGL((mx_slice_kernel<FX, DT, MT, NT>), dim3(tm * ai4e_cdiv(n, 16 * NT)), dim3(SLICES * 64), 0, s,
                      static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), static_cast<const uint8_t*>(w),
                      static_cast<const uint8_t*>(ws), static_cast<const float*>(bias), m, n, kp, tm,
@@ -758,15 +757,21 @@ int launch(const void* x, const void* xs, const void* w, const void* ws, const v
 #undef ARGS
 }
 
+// What a launch of fewer than 2^32 threads holds: 2^22 tiles of 128 x 128; of slices (`launch`: short k, few rows or
+// outputs) fewer than 2^23 of 32 x 64.
+bool fits(int m, int n, int kp) {
+  const auto blocks = [&](int bm, int bn) { return static_cast<long>(ai4e_cdiv(m, bm)) * ai4e_cdiv(n, bn); };
+  return kp <= (1 << 23) && n <= (1 << 30) && m <= (1 << 30) && blocks(128, 128) <= (1L << 22) &&
+         (kp >= 512 || (m > 32 && n >= 4) || blocks(32, 64) < (1L << 23));
+}
+
 }  // namespace
 
 // x: data [m, kp] (fx 0, e4m3) or [m, kp / 2] (fx 1, e2m1), xs [m, kp / 32]; w: [n, kp / 2], ws [n, kp / 32];
 // bias [n] fp32 or null; y [m, n] of type dt (0 bf16, 1 fp16, 2 fp32). kp is a multiple of 128.
 AI4E_API int ai4e_mx_linear(const void* x, const void* xs, int fx, const void* w, const void* ws, const void* bias,
                             int m, int n, int kp, void* y, int dt, hipStream_t s) {
-  if (m < 0 || n <= 0 || kp <= 0 || kp % MX_ALIGN || fx < 0 || fx > 1 || dt < 0 || dt > 2 ||
-      kp > (1 << 23) || n > (1 << 30) || m > (1 << 30) || static_cast<long>(ai4e_cdiv(m, 128)) * ai4e_cdiv(n, 128) > (1L << 22))
-    return AI4E_EINVAL;
+  if (m < 0 || n <= 0 || kp <= 0 || kp % MX_ALIGN || fx < 0 || fx > 1 || dt < 0 || dt > 2 || !fits(m, n, kp)) return AI4E_EINVAL;
   if (m == 0) return AI4E_OK;  // tensors without elements have no memory
   if (!x || !xs || !w || !ws || !y) return AI4E_EINVAL;
 #define GO(FX, DT) return launch<FX, DT>(x, xs, w, ws, bias, m, n, kp, y, s)

@@ -3,8 +3,9 @@ import pytest
 import torch
 
 import lm_oracle as oracle
-from aiforearth_api_platform_amd.ops import _ext
-from aiforearth_api_platform_amd.ops.mx import mx_dequantize
+from aiforearth_api_platform_amd.ops import _ext, mx
+from aiforearth_api_platform_amd.ops.head import label_logprobs
+from aiforearth_api_platform_amd.ops.mx import MxTensor, mx_dequantize, mx_linear, mx_quantize
 from aiforearth_api_platform_amd.ops.norm import rms_norm_mx8
 
 
@@ -54,3 +55,48 @@ def test_rms_norm_reference_takes_the_kernels_sums(dtype):
     x, r = torch.full((2, 64), 4.25, dtype=dtype), torch.full((2, 64), 2.0 ** -23, dtype=dtype)
     q, h = rms_norm_mx8(x, torch.ones(64), r, 2.0 ** 40)
     assert mx_dequantize(q).eq(4 * 2.0 ** -20).all() and h.eq(4.25).all()
+
+
+def shapes_only(rows, k):
+    """An e2m1 MxTensor without memory behind it."""
+    kp = mx.padded(k)
+    return MxTensor(torch.empty(rows, kp // 2, dtype=torch.uint8, device="meta"),
+                    torch.empty(rows, kp // 32, dtype=torch.uint8, device="meta"), k)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1, (1 << 23) + 1),           # deeper than 2^23
+                                   ((1 << 29) + 1, 1, 512),         # over 2^22 tiles of 128 x 128
+                                   (1 << 20, 1 << 17, 128),
+                                   ((1 << 31) + 7, 1, 128), ((1 << 32) + 7, 1, 128),
+                                   (1 << 28, 3, 100),               # 2^23 or more slices of 32 x 64
+                                   (32, 1 << 29, 384)])
+def test_linear_refuses_more_than_a_launch_holds(m, n, k):
+    with pytest.raises(ValueError):
+        mx_linear(shapes_only(m, k), shapes_only(n, k))
+    if m < 1 << 31 and n < 1 << 31:
+        assert kernels().ai4e_mx_linear(16, 16, 1, 16, 16, None, m, n, mx.padded(k), 16, 0, None) == 1
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 3, 1 << 23), (1 << 29, 4, 128), ((1 << 28) - 32, 3, 100), (32, (1 << 29) - 64, 384)])
+def test_linear_takes_what_a_launch_holds(m, n, k):
+    assert mx._linear_fits(m, n, mx.padded(k))
+
+
+def test_quantize_refuses_more_than_a_launch_holds():
+    rows = ((1 << 33) - 512) // 16  # of 16 groups of 8 values
+    lib = kernels()
+    x = torch.empty(rows + 1, 100, dtype=torch.bfloat16, device="meta")
+    with pytest.raises(ValueError):
+        mx_quantize(x)
+    with pytest.raises(ValueError):
+        mx_dequantize(shapes_only(rows + 1, 100))
+    assert mx_quantize(x[1:]).shape == mx_dequantize(shapes_only(rows, 100)).shape == (rows, 100)
+    assert lib.ai4e_mx_quantize(16, 100, rows + 1, 100, 0, 1, 16, 16, None) == 1
+    assert lib.ai4e_mx_dequantize(16, 16, rows + 1, 100, 0, 1, 16, None) == 1
+
+
+def test_label_logprobs_refuses_more_labels_than_an_int_counts():
+    for n in ((1 << 30) + 1, (1 << 32) + 3):
+        with pytest.raises(ValueError):
+            label_logprobs(torch.empty(8, device="meta"), torch.empty(n, dtype=torch.int32, device="meta"), 1)
+    assert kernels().ai4e_label_logprobs(16, 8, 1, 8, 0, 16, 0, (1 << 30) + 1, 1, 16, 16, 16, 16, None) == 1
