@@ -16,6 +16,7 @@ from pathlib import Path
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB_PATH = Path(__file__).resolve().parent.parent / "_lib" / "libai4e_kernels.so"
 if os.environ.get("AI4E_KERNEL_LIB"):  # A/B of two builds of the kernel library on one GPU box
@@ -152,9 +153,13 @@ def call_on(index: int, name: str, *args) -> None:
 
 
 def refuse_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    """For operators with no backward pass: a call that autograd would have to record is an error."""
+    """For operators with no derivative: a call that autograd would have to record, or whose inputs carry a tangent, is an
+    error."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                            for t in tensors):  # within a dual_level only
+        raise ValueError(f"{name} has no forward-mode derivative: call it on detached tensors")
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

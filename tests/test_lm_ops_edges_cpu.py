@@ -1,6 +1,7 @@
 """Language-model operators at the edges of what their documents allow, without a GPU."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import lm_oracle as oracle
 from aiforearth_api_platform_amd.ops import _ext, mx
@@ -100,3 +101,19 @@ def test_label_logprobs_refuses_more_labels_than_an_int_counts():
         with pytest.raises(ValueError):
             label_logprobs(torch.empty(8, device="meta"), torch.empty(n, dtype=torch.int32, device="meta"), 1)
     assert kernels().ai4e_label_logprobs(16, 8, 1, 8, 0, 16, 0, (1 << 30) + 1, 1, 16, 16, 16, 16, None) == 1
+
+
+def test_forward_mode_derivatives_are_refused():
+    """No operator has a derivative, in either direction: a tangent would be lost without a word."""
+    x, ones = torch.randn(2, 64), torch.ones(64)
+    q, w = mx_quantize(x), mx_quantize(torch.randn(64, 64))
+    with forward_ad.dual_level():
+        dual, dual1 = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(ones, ones.clone())
+        for call in (lambda: mx_quantize(dual), lambda: rms_norm_mx8(dual, ones), lambda: rms_norm_mx8(x, dual1),
+                     lambda: rms_norm_mx8(x, ones, dual), lambda: mx_linear(q, w, dual1), lambda: label_logprobs(dual)):
+            for grad in (torch.enable_grad, torch.no_grad):  # no_grad stops the other direction only
+                with grad(), pytest.raises(ValueError):
+                    call()
+        # a tensor without a tangent, and one that was detached from it
+        rms_norm_mx8(x, ones, dual.detach())
+        label_logprobs(x, None, 1)
