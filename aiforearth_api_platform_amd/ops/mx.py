@@ -158,6 +158,7 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
     check("mx_dequantize", q)
     if dtype not in DTYPE_CODE:
         raise ValueError("mx_dequantize gives bfloat16, float16 or float32")
+    _ext.refuse_grad("mx_dequantize", q.data, q.scale)
     _check_rows("mx_dequantize", q.scale.numel() // q.scale.shape[-1], q.k)
     if _ext.backend_for(q.data) != "hip":
         return dequantize_reference(q).to(dtype)
@@ -205,7 +206,7 @@ def mx_linear(x: MxTensor, w: MxTensor, bias: Optional[torch.Tensor] = None,
     index = data.get_device()
     if w.data.get_device() != index or (bias is not None and bias.get_device() != index):
         raise ValueError("mx_linear: x, w and bias have to be on one device")
-    _ext.refuse_grad("mx_linear", bias)
+    _ext.refuse_grad("mx_linear", data, scale, w.scale, bias)
     if _ext.backend_for(data) != "hip":
         y = dequantize_reference(x) @ dequantize_reference(w).T
         return (y if bias is None else y + bias.float()).to(out_dtype)

@@ -117,3 +117,15 @@ def test_forward_mode_derivatives_are_refused():
         # a tensor without a tangent, and one that was detached from it
         rms_norm_mx8(x, ones, dual.detach())
         label_logprobs(x, None, 1)
+
+
+def test_codes_that_require_a_gradient_are_refused():
+    q, w = mx_quantize(torch.randn(2, 64), "e4m3"), mx_quantize(torch.randn(5, 64))
+    leaf = [MxTensor(q.data.clone().requires_grad_(), q.scale, 64), MxTensor(q.data, q.scale.clone().requires_grad_(), 64)]
+    scaled = MxTensor(w.data, w.scale.clone().requires_grad_(), 64)
+    for call in (*[lambda t=t: mx_dequantize(t) for t in leaf], *[lambda t=t: mx_linear(t, w) for t in leaf],
+                 lambda: mx_linear(q, scaled)):
+        with pytest.raises(ValueError):
+            call()
+        with torch.no_grad():
+            call()
