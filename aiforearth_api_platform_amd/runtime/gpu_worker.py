@@ -108,12 +108,12 @@ def pin_host(buf: torch.Tensor) -> bool:
         rc = torch.cuda.cudart().cudaHostRegister(buf.data_ptr(), buf.numel(), 0)
         if (int(rc[0]) if isinstance(rc, tuple) else int(rc)) == 0:
             return True
+        from ..ops import _ext
+
+        if _ext.available() and _ext.has("ai4e_clear_error"):
+            _ext.call_int("ai4e_clear_error")
     except Exception:
         pass
-    from ..ops import _ext
-
-    if _ext.available():
-        _ext.call_int("ai4e_clear_error")
     return False
 
 
