@@ -768,17 +768,18 @@ bool fits(int m, int n, int kp) {
 }  // namespace
 
 // x: data [m, kp] (fx 0, e4m3) or [m, kp / 2] (fx 1, e2m1), xs [m, kp / 32]; w: [n, kp / 2], ws [n, kp / 32];
-// bias [n] fp32 or null; y [m, n] of type dt (0 bf16, 1 fp16, 2 fp32). kp is a multiple of 128.
+// bias [n] fp32 or null; y [m, n] of type dt (0 bf16, 1 fp16, 2 fp32: of e2m1 x only). kp is a multiple of 128.
 AI4E_API int ai4e_mx_linear(const void* x, const void* xs, int fx, const void* w, const void* ws, const void* bias,
                             int m, int n, int kp, void* y, int dt, hipStream_t s) {
-  if (m < 0 || n <= 0 || kp <= 0 || kp % MX_ALIGN || fx < 0 || fx > 1 || dt < 0 || dt > 2 || !fits(m, n, kp)) return AI4E_EINVAL;
+  if (m < 0 || n <= 0 || kp <= 0 || kp % MX_ALIGN || fx < 0 || fx > 1 || dt < 0 || dt > 2 ||
+      (fx == MX_E4M3 && dt == MX_F32) || !fits(m, n, kp))
+    return AI4E_EINVAL;
   if (m == 0) return AI4E_OK;  // tensors without elements have no memory
   if (!x || !xs || !w || !ws || !y) return AI4E_EINVAL;
 #define GO(FX, DT) return launch<FX, DT>(x, xs, w, ws, bias, m, n, kp, y, s)
   if (fx == MX_E4M3) {
     if (dt == MX_BF16) GO(MX_E4M3, MX_BF16);
-    if (dt == MX_F16) GO(MX_E4M3, MX_F16);
-    GO(MX_E4M3, MX_F32);
+    GO(MX_E4M3, MX_F16);
   }
   if (dt == MX_BF16) GO(MX_E2M1, MX_BF16);
   if (dt == MX_F16) GO(MX_E2M1, MX_F16);

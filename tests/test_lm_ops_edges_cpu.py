@@ -129,3 +129,8 @@ def test_codes_that_require_a_gradient_are_refused():
             call()
         with torch.no_grad():
             call()
+
+
+def test_c_entry_refuses_32_bit_results_of_8_bit_operands():
+    """As the public function does: such products are added to about 17 bits."""
+    assert kernels().ai4e_mx_linear(16, 16, 0, 16, 16, None, 1, 4, 128, 16, 2, None) == 1
