@@ -155,11 +155,15 @@ def call_on(index: int, name: str, *args) -> None:
 def refuse_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
     """For operators with no derivative: a call that autograd would have to record, or whose inputs carry a tangent, is an
     error."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
-    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
-                                                            for t in tensors):  # within a dual_level only
-        raise ValueError(f"{name} has no forward-mode derivative: call it on detached tensors")
+    record, dual = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    if record or dual:
+        for t in tensors:
+            if t is None:
+                continue
+            if record and t.requires_grad:
+                raise ValueError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+            if dual and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode derivative: call it on detached tensors")
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

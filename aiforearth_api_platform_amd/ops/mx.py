@@ -130,9 +130,8 @@ def dequantize_reference(q: MxTensor) -> torch.Tensor:
     return (v.reshape(*code.shape, BLOCK) * s[..., None]).reshape(v.shape)[..., :q.k]
 
 
-def _check_rows(name: str, rows: int, k: int) -> None:
-    if rows * (padded(k) // 8) > (1 << 33) - 512:  # a launch has fewer than 2^32 threads, of 16 values each
-        raise ValueError(f"{name}: rows of {k} are taken up to {((1 << 33) - 512) // (padded(k) // 8)} at once, not {rows}")
+# scale bytes of a launch of quantisation, which has fewer than 2^32 threads, of 16 values each
+MAX_SCALES = (1 << 31) - 128
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "e2m1") -> MxTensor:
@@ -142,7 +141,9 @@ def mx_quantize(x: torch.Tensor, fmt: str = "e2m1") -> MxTensor:
     if x.dtype not in DTYPE_CODE or x.dim() < 1 or not 0 < x.shape[-1] <= MAX_WIDTH:
         raise ValueError("mx_quantize expects bfloat16, float16 or float32 with a last axis of 1 to 2^30 values")
     _ext.refuse_grad("mx_quantize", x)
-    _check_rows("mx_quantize", x.numel() // x.shape[-1], x.shape[-1])
+    # rows of one value, stored as 128, reach the limit first
+    if x.numel() >= 1 << 28 and x.numel() // x.shape[-1] * (padded(x.shape[-1]) // BLOCK) > MAX_SCALES:
+        raise ValueError(f"mx_quantize: {tuple(x.shape)} are over 2^36 stored values")
     if _ext.backend_for(x) != "hip":
         return quantize_reference(x, fmt)
     k = x.shape[-1]
@@ -159,7 +160,8 @@ def mx_dequantize(q: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
     if dtype not in DTYPE_CODE:
         raise ValueError("mx_dequantize gives bfloat16, float16 or float32")
     _ext.refuse_grad("mx_dequantize", q.data, q.scale)
-    _check_rows("mx_dequantize", q.scale.numel() // q.scale.shape[-1], q.k)
+    if q.scale.numel() > MAX_SCALES:
+        raise ValueError(f"mx_dequantize: {tuple(q.shape)} are over 2^36 stored values")
     if _ext.backend_for(q.data) != "hip":
         return dequantize_reference(q).to(dtype)
     y = new(q.shape, dtype, q.data.device)
@@ -200,7 +202,7 @@ def mx_linear(x: MxTensor, w: MxTensor, bias: Optional[torch.Tensor] = None,
     if bias is not None and (tuple(bias.shape) != (n,) or not bias.is_floating_point()):
         raise ValueError(f"mx_linear: bias is a floating tensor of {n} values")
     m = scale.numel() // scale.shape[-1]
-    if not _linear_fits(m, n, padded(k)):
+    if (m > 1 << 15 or n > 1 << 18 or k > 1 << 23) and not _linear_fits(m, n, padded(k)):  # smaller ones do
         raise ValueError(f"mx_linear: {m} rows of {k} by {n} outputs are more than a launch holds (k up to 2^23, 2^22 tiles of "
                          "128 rows by 128 outputs)")
     index = data.get_device()
