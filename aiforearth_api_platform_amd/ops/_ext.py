@@ -23,7 +23,7 @@ if os.environ.get("AI4E_KERNEL_LIB"):  # A/B of two builds of the kernel library
     _LIB_PATH = Path(os.environ["AI4E_KERNEL_LIB"])
 _lib: Optional[ctypes.CDLL] = None
 
-_c_int, _c_long, _c_float, _c_double, _vp = ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_double, ctypes.c_void_p
+_c_int, _c_long, _c_float, _vp = ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_void_p
 
 # name -> argtypes (all return int status)
 _SIGS = {
@@ -78,7 +78,7 @@ _SIGS = {
     "ai4e_mx_quantize": [_vp, _c_long, _c_long, _c_int, _c_int, _c_int, _vp, _vp, _vp],
     "ai4e_mx_dequantize": [_vp, _vp, _c_long, _c_int, _c_int, _c_int, _vp, _vp],
     "ai4e_mx_linear": [_vp, _vp, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int, _vp],
-    "ai4e_rms_norm_mx8": [_vp, _c_long, _vp, _c_long, _vp, _c_double, _c_long, _c_int, _c_int, _vp, _vp, _vp, _vp],
+    "ai4e_rms_norm_mx8": [_vp, _c_long, _vp, _c_long, _vp, _c_float, _c_long, _c_int, _c_int, _vp, _vp, _vp, _vp],
     "ai4e_label_logprobs": [_vp, _c_long, _c_long, _c_int, _c_int, _vp, _c_int, _c_int, _c_int] + [_vp] * 5,
     "ai4e_crumbs_alloc": [_c_int, _vp, _vp],
     "ai4e_crumb": [_vp, _c_int, _vp],

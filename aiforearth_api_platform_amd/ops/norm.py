@@ -2,6 +2,7 @@
 residual's addition, written as MX e4m3."""
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -161,7 +162,7 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
     ``mx.mx_linear`` (csrc/kernels/rms_norm.hip). ``x`` and ``residual`` [..., C] in bf16, fp16 or fp32 (rows may be
     strided), ``gamma`` [C] (kept in float32 by a caller that wants no cast per call). Returns the MxTensor and ``h`` in
     x's type, for the next residual (None without ``residual``); the norm is taken of the sum before that rounding: of the
-    32-bit sum of 16-bit rows, of the exact sum of 32-bit ones."""
+    32-bit sum of 16-bit rows, of the exact sum of 32-bit ones. ``eps`` is rounded to 32 bits."""
     c = x.shape[-1] if x.dim() else 0
     if x.dtype not in mx.DTYPE_CODE or not 0 < c <= mx.MAX_WIDTH:
         raise ValueError("rms_norm_mx8 expects bfloat16, float16 or float32 with a last axis of 1 to 2^30 values")
@@ -172,8 +173,9 @@ def rms_norm_mx8(x: torch.Tensor, gamma: torch.Tensor, residual: Optional[torch.
         raise ValueError(f"rms_norm_mx8: gamma is a floating tensor of {c} values")
     if gamma.get_device() != index or (residual is not None and residual.get_device() != index):
         raise ValueError("rms_norm_mx8: x, gamma and residual have to be on one device")
-    if not eps >= 2.0 ** -149:  # from there on a row's factor is a 32-bit number, whatever the row holds
-        raise ValueError("rms_norm_mx8: eps has to be positive, 2^-149 or more")
+    eps = ctypes.c_float(eps).value
+    if not eps > 0:
+        raise ValueError("rms_norm_mx8: eps has to be positive, in 32 bits")
     _ext.refuse_grad("rms_norm_mx8", x, gamma, residual)
     if _ext.backend_for(x) != "hip":
         h = x.float() if residual is None else x.float() + residual.float()

@@ -69,7 +69,7 @@ __device__ __forceinline__ void load_h(const typename mx_elem<DT>::type* x, cons
 template <int DT, int LANES, int CH>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_mx8_kernel(
     const typename mx_elem<DT>::type* __restrict__ x, long ldx, const typename mx_elem<DT>::type* __restrict__ res,
-    long ldr, const float* __restrict__ gamma, double eps, double inv_c, long rows, int c, int cp,
+    long ldr, const float* __restrict__ gamma, float eps, double inv_c, long rows, int c, int cp,
     typename mx_elem<DT>::type* __restrict__ hout, uint8_t* __restrict__ data, uint8_t* __restrict__ scale) {
   constexpr int T = LANES > 256 ? LANES : 256, ROWS = T / LANES;
   static_assert(LANES <= 64 || ROWS == 1, "rows of several waves share no workgroup: they meet at its barriers");
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_mx8_kernel
       }
       if (hout) mx_store8_quad<DT>(hout + row * c, col, c, v);
     }
-    const double factor = inv_sqrt(row_sum<LANES>(sq, lds) * inv_c + eps);
+    const double factor = inv_sqrt(row_sum<LANES>(sq, lds) * inv_c + static_cast<double>(eps));
     const float fh = static_cast<float>(factor), fl = static_cast<float>(factor - static_cast<double>(fh));
 #pragma unroll
     for (int j = 0; j < nch; ++j) {
@@ -147,9 +147,9 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void rms_norm_mx8_kernel
 
 // x [rows, ldx] and residual [rows, ldr] (or null) of type dt (0 bf16, 1 fp16, 2 fp32), c valid columns; gamma [c] fp32;
 // hout [rows, c] of type dt (or null); data [rows, cp], scale [rows, cp / 32], cp = c up to a multiple of 128.
-AI4E_API int ai4e_rms_norm_mx8(const void* x, long ldx, const void* residual, long ldr, const void* gamma, double eps,
+AI4E_API int ai4e_rms_norm_mx8(const void* x, long ldx, const void* residual, long ldr, const void* gamma, float eps,
                                long rows, int c, int dt, void* hout, void* data, void* scale, hipStream_t s) {
-  if (c <= 0 || c > (1 << 30) || rows < 0 || dt < 0 || dt > 2 || ldx < c || (residual && ldr < c) || !(eps >= 0x1p-149))
+  if (c <= 0 || c > (1 << 30) || rows < 0 || dt < 0 || dt > 2 || ldx < c || (residual && ldr < c) || !(eps > 0.f))
     return AI4E_EINVAL;
   if (rows == 0) return AI4E_OK;  // tensors without elements have no memory
   if (!x || !gamma || !data || !scale) return AI4E_EINVAL;

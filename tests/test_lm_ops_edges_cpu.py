@@ -37,17 +37,21 @@ def test_rms_norm_refuses_an_eps_that_32_bits_do_not_hold(eps):
 
 
 def test_rms_norm_reference_rounds_once():
-    """y lies below the border 1.1875 of 1.125 and 1.25 by less than 32 bits hold: it becomes 1.125."""
-    eps = 2.0 ** -20 * (1 + 2.0 ** -25)
-    x, gamma = torch.full((2, 40), 2.0 ** -40), torch.full((40,), 1.1875)
+    """y lies next to a border, 1.1875 of 1.125 and 1.25 or 1.0625 of 1 and 1.125, by less than 32 bits hold."""
+    x = torch.full((2, 40), 2.0 ** -24)  # the squares are 2^-28 of eps
     x[1] *= -1
-    want = oracle.mx_values(oracle.rms_norm(x, gamma, None, eps), "e4m3")
-    assert want[0].eq(1.125 * 2.0 ** -30).all()
-    assert torch.equal(mx_dequantize(rms_norm_mx8(x, gamma, None, eps)[0]).double(), want)
-    # above the border between 1 and 1.125, which falls to 1; at one it stays there
-    gamma[:] = 1.0625
-    for e, value in ((2.0 ** -20 * (1 - 2.0 ** -25), 1.125), (2.0 ** -20, 1.0)):
-        assert mx_dequantize(rms_norm_mx8(x, gamma, None, e)[0])[0].eq(value * 2.0 ** -30).all()
+    for gamma, eps, value in ((1.1875, 2.0 ** -20, 1.125), (1.0625, 2.0 ** -20 * (1 - 2.0 ** -24), 1.125), (1.0625, 2.0 ** -20, 1.0)):
+        g = torch.full((40,), gamma)
+        want = oracle.mx_values(oracle.rms_norm(x, g, None, eps), "e4m3")
+        assert want[0].eq(value * 2.0 ** -14).all()
+        assert torch.equal(mx_dequantize(rms_norm_mx8(x, g, None, eps)[0]).double(), want)
+
+
+def test_rms_norm_eps_is_a_32_bit_number():
+    """As it is in the kernel: what 32 bits do not hold of it moves no element."""
+    x, gamma = torch.full((2, 40), 2.0 ** -40), torch.full((40,), 1.1875)  # at the border, which falls to 1.25
+    for eps in (2.0 ** -20, 2.0 ** -20 * (1 + 2.0 ** -25), 2.0 ** -20 * (1 - 2.0 ** -26)):
+        assert mx_dequantize(rms_norm_mx8(x, gamma, None, eps)[0]).eq(1.25 * 2.0 ** -30).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])

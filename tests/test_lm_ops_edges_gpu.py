@@ -103,18 +103,20 @@ def test_no_rows(shape):
 
 
 @pytest.mark.parametrize("c", [64, 3000, 20000])
-def test_rms_norm_eps_is_not_rounded(c):
-    """Where eps outweighs the squares, y is x / sqrt(eps) * gamma. 1.1875 is the border between 1.125 and 1.25 and falls to
-    the latter; what 32 bits do not hold of this eps takes y below it."""
-    eps = 2.0 ** -20 * (1 + 2.0 ** -25)
-    x = torch.full((3, c), 2.0 ** -40)
+def test_rms_norm_where_eps_outweighs_the_squares(c):
+    """y is next to a border by less than 32 bits hold, below it and above. eps itself is a 32-bit number on both devices."""
+    x = torch.full((3, c), 2.0 ** -24)  # the squares are 2^-28 of eps
     x[1] = -x[1]
-    gamma = torch.full((c,), 1.1875)
-    q, _ = rms_norm_mx8(x.to(DEV), gamma.to(DEV), None, eps)
-    want = oracle.mx_values(oracle.rms_norm(x, gamma, None, eps), "e4m3")
-    assert want[0].eq(1.125 * 2.0 ** -30).all() and torch.equal(mx_dequantize(q).cpu().double(), want)
-    q, _ = rms_norm_mx8(x * 2.0 ** -30, gamma, None, 2.0 ** -149)
-    p, _ = rms_norm_mx8((x * 2.0 ** -30).to(DEV), gamma.to(DEV), None, 2.0 ** -149)
+    for gamma, eps, value in ((1.1875, 2.0 ** -20, 1.125), (1.0625, 2.0 ** -20 * (1 - 2.0 ** -24), 1.125), (1.0625, 2.0 ** -20, 1.0)):
+        g = torch.full((c,), gamma)
+        assert oracle.mx_values(oracle.rms_norm(x, g, None, eps), "e4m3")[0].eq(value * 2.0 ** -14).all()
+        for dev in ("cpu", DEV):
+            for e in (eps, eps * (1 + 2.0 ** -27), eps * (1 - 2.0 ** -27)):
+                q, _ = rms_norm_mx8(x.to(dev), g.to(dev), None, e)
+                assert mx_dequantize(q)[[0, 2]].eq(value * 2.0 ** -14).all() and mx_dequantize(q)[1].eq(-value * 2.0 ** -14).all()
+    tiny = x * 2.0 ** -46
+    q, _ = rms_norm_mx8(tiny, g, None, 2.0 ** -149)
+    p, _ = rms_norm_mx8(tiny.to(DEV), g.to(DEV), None, 2.0 ** -149)
     assert torch.equal(mx_dequantize(p).cpu(), mx_dequantize(q))
 
 
