@@ -162,8 +162,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const bool in = (pmask >> k) & 1u;
       uint4 v = in ? pv[k] : make_uint4(0u, 0u, 0u, 0u);
       if (p.pro != nullptr && in) {  // padding stays zero: the conv pads the normalized tensor
-        // packed math per channel pair: one v_pk_fma_f32, one v_cvt_pk_bf16_f32 and (ReLU) one v_pk_max_i16 on the
-        // packed bf16 (relu(round(x)) == round(relu(x))), instead of two FMAs, two max and a pack
+        // per channel pair two FMAs, one v_cvt_pk_bf16_f32 and (ReLU) one v_pk_max_i16 on the packed bf16
+        // (relu(round(x)) == round(relu(x))), instead of two FMAs, two max and a pack
         uint32_t wds[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {

@@ -154,7 +154,7 @@ __device__ __forceinline__ int mx_scale_code(uint32_t amax) {
   return e == 255 ? 255 : max(code, 0);
 }
 
-// 2^(127 - code); 0..247 are all the codes of finite blocks
+// 2^(127 - code); finite blocks have codes up to 247 (e4m3) or 253 (e2m1)
 __device__ __forceinline__ float mx_inv_scale(int code) {
   return __uint_as_float(static_cast<uint32_t>(254 - code) << 23);
 }

@@ -3,7 +3,8 @@
 // y = round(x / 2^e) per block of 32, e from the block's largest |x|: nothing but a maximum over 32 values stands between
 // a load and a store, so both directions are bound by memory. A thread takes 8 values (16 B of 16-bit input) twice, four
 // neighbouring lanes a block: the maximum is two DPP steps, and a wave's stores are contiguous. 16384 x 8192 bf16 to e2m1
-// 59 us (5.75 TB/s; 67 with one group per thread, 60 with four), back 48 us (through L2 108).
+// 59 us (5.75 TB/s; 67 with one group per thread, 60 with four), back 66 us with the codes out of memory (5.2 TB/s) and 48
+// where the memory-side cache still holds them (through L2 108).
 #include "mx.h"
 
 namespace {
