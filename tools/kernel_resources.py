@@ -10,7 +10,7 @@ import sys
 src = sys.argv[1]
 flt = sys.argv[2] if len(sys.argv) > 2 else ""
 cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-munsafe-fp-atomics",
-       "-mllvm", "-amdgpu-mfma-vgpr-form=1", "-Icsrc/kernels", "-c", src, "-o", "/tmp/_kres.o",
+       "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-mllvm", "-amdgpu-mfma-vgpr-form=1", "-Icsrc/kernels", "-c", src, "-o", "/tmp/_kres.o",
        "-Rpass-analysis=kernel-resource-usage"]
 out = subprocess.run(cmd, capture_output=True, text=True).stderr
 rows, cur = [], None
